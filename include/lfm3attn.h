@@ -43,7 +43,11 @@ enum {
   LFM3A_MODE_F16 = 0,
   /* The reference's int8 records: per (slot, kv head) K int8[D] | K scale f32 | V int8[D] |
    * V scale f32 (kernels/ops.hip:226-251, internal/model/engine.go:28-32). */
-  LFM3A_MODE_I8REC = 1
+  LFM3A_MODE_I8REC = 1,
+  /* 8-bit K and V with one scale per 32-token block and kv head, int8 or fp8 e4m3 (no reference counterpart):
+   * the caches of the lfm3a_kv8_* calls. */
+  LFM3A_MODE_I8BLK = 2,
+  LFM3A_MODE_E4M3BLK = 3
 };
 
 /* Geometry and strides of one layer's paged pool. */
@@ -52,7 +56,7 @@ typedef struct lfm3a_kv_layout {
   int32_t kv_heads;      /* 8 (benchmark geometry) or 4 (the reference model) */
   int32_t head_dim;      /* 64 or 128 */
   int32_t block_tokens;  /* tokens per block: 32, as engine.go:31 (BlockTokens) */
-  int64_t head_bytes;    /* MODE_F16: bytes of one (block, kv head) section; MODE_I8REC: record bytes */
+  int64_t head_bytes;    /* bytes of one (block, kv head) section; MODE_I8REC: record bytes */
   int64_t block_bytes;   /* bytes of one block, all kv heads (engine.go:32 KVBlock for MODE_I8REC) */
 } lfm3a_kv_layout;
 
@@ -448,6 +452,86 @@ int64_t lfm3a_g128_workspace_bytes(int rows, int k);
 int lfm3a_g128_linear(const void* x, int64_t x_stride, int rows, int gated, const void* w, const float* w_scales,
                       int outputs, int k, const void* residual, int64_t residual_stride, void* out,
                       int64_t out_stride, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------- 8-bit block cache (MODE_I8BLK, MODE_E4M3BLK)
+ * No reference counterpart: half the bytes of MODE_F16 per cached token, and no scale per token. A block (32 tokens) is
+ * sealed once it is complete and committed: K and V of each kv head are held as q = round8(x / s), the quotient in
+ * fp32, rounded to nearest even and saturated to int8 (-127 .. 127) or e4m3 (+-448), with one fp32 scale
+ * s = absmax / 127 (or / 448; 1 for a block of zeros) per block, kv head and K or V. The tokens past the sealed ones
+ * stay in fp16 in the tail, a ring of 128 tokens per layer, so drafts that are rolled back never touch sealed bytes
+ * and a rollback needs no device work. Calls take `sealed`, the number of sealed tokens (a multiple of 32); at most
+ * 128 tokens lie past it. Cached values are finite: NaN is stored as 0, an infinity as +-65504. */
+typedef struct lfm3a_kv8_view {
+  lfm3a_kv_view kv;   /* pool and block table of a MODE_I8BLK or MODE_E4M3BLK layout (sealed blocks) */
+  void* tail;         /* device: lfm3a_kv8_tail_bytes bytes */
+} lfm3a_kv8_view;
+
+/* Bytes of a layer's tail: K [kv_heads][128 slots][head_dim], then V [kv_heads][head_dim][128 slots], fp16, the slot of
+ * a position being position mod 128. 0 for another mode. */
+size_t lfm3a_kv8_tail_bytes(const lfm3a_kv_layout* layout);
+
+/* Stores n tokens at pos0 .. pos0 + n - 1 (k, v, token_stride, rope, k_norm as lfm3a_kv_append; the same fp16 K) and
+ * seals every block that lies wholly below seal_to (sealed <= seal_to <= pos0 + n): afterwards
+ * seal_to / 32 * 32 tokens are sealed. Tokens sealed .. pos0 - 1 must be in the tail. A prompt chunk passes
+ * seal_to = pos0 + n; a round of drafts passes seal_to = pos0, the tokens committed so far. n = 0 only seals. */
+int lfm3a_kv8_append(const lfm3a_kv8_view* kv, const void* k, const void* v, int64_t token_stride, int pos0, int n,
+                     int sealed, int seal_to, const void* rope, const void* k_norm, void* stream);
+
+/* The values that tokens pos0 .. pos0 + n - 1 stand for, rounded to fp16: k, v device [n][kv_heads][head_dim]. */
+int lfm3a_kv8_read(const lfm3a_kv8_view* kv, int pos0, int n, int sealed, void* k, void* v, void* stream);
+
+/* Most query rows (m * q_heads / kv_heads) of an lfm3a_kv8_attention or lfm3a_kv8_weights call. */
+#define LFM3A_KV8_MAX_ROWS 256
+
+/* The key split count lfm3a_kv8_attention uses when called with splits <= 0. */
+int lfm3a_kv8_splits(const lfm3a_kv_layout* layout, int q_heads, int ctx_len, int m, int window, int sm_count);
+
+/* Attention of m tokens at ctx_len .. ctx_len + m - 1 over the cache [0, ctx_len + m): a decoded token, a round of
+ * drafts (appended before, in the tail) or a short prompt chunk. Token t sees the keys up to ctx_len + t, and with
+ * window > 0 only the last `window` of them. q: device fp16, row (t, qh) at q + t * q_stride + qh * head_dim (q_stride in halves, a
+ * multiple of 8; 0: contiguous). gate: device fp16 [m][q_heads] logits (out *= sigmoid) or NULL. out: device fp16
+ * [m][q_heads][head_dim]. lse: device fp32 [m][q_heads], the natural logarithm of each row's sum of exponentials, or
+ * NULL. q_heads: any multiple of kv_heads; 1 <= m <= 32 and m * q_heads / kv_heads <= 256; head_dim 64 or 128.
+ * workspace: lfm3a_verify_workspace_bytes(m, q_heads, head_dim, splits) bytes when splits > 1. */
+int lfm3a_kv8_attention(const lfm3a_kv8_view* kv, const void* q, int64_t q_stride, int m, int q_heads, int ctx_len,
+                        int sealed, int window, const void* gate, void* out, float* lse, void* workspace,
+                        size_t workspace_bytes, int splits, void* stream);
+
+/* Attention of a prompt chunk of any length (appended before) at context .. context + tokens - 1, causal, optionally
+ * sliding-window; q, out as above. The blocks that the chunk sees are staged as fp16 in the workspace for the kernel of
+ * lfm3a_prefill_attention(exact = 1); a chunk of up to 32 tokens, or a GQA group other than 4, goes through
+ * lfm3a_kv8_attention 32 tokens at a time. workspace: lfm3a_kv8_prefill_workspace_bytes bytes for the sequence's length
+ * (or more; less splits fewer keys or fails with LFM3A_EWORKSPACE). */
+size_t lfm3a_kv8_prefill_workspace_bytes(const lfm3a_kv_layout* layout, int tokens, int q_heads, int max_len);
+int lfm3a_kv8_prefill(const lfm3a_kv8_view* kv, const void* q, int64_t q_stride, int tokens, int q_heads, int context,
+                      int sealed, int window, void* out, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------- eviction by accumulated attention weight
+ * No reference counterpart. Per layer: lfm3a_kv8_weights after the attention of a round (or of a prompt's last
+ * tokens) adds up how much each cached key was attended to; lfm3a_evict_select picks the keys to keep, per kv head;
+ * lfm3a_kv8_compact moves them into a smaller cache, in which attention goes on with window = 0 (a key's slot is no
+ * longer its position; its RoPE rotation stays, so later appends pass the table's row of the true position). */
+
+/* out[h][key] = decay * prev[h][key] + sum over the m tokens t and the query heads of kv head h of exp(s - lse[t][qh]),
+ * s = q . k / sqrt(head_dim), over the keys that token t sees, for the keys 0 .. ctx_len + m - 1. lse: of
+ * lfm3a_kv8_attention for the same q. prev (row stride prev_stride floats; NULL: no older sum) may be out itself. Keys appended since
+ * prev was made need rows that hold 0 for them. Arguments otherwise as lfm3a_kv8_attention. */
+int lfm3a_kv8_weights(const lfm3a_kv8_view* kv, const void* q, int64_t q_stride, int m, int q_heads, int ctx_len,
+                      int sealed, int window, const float* lse, const float* prev, int64_t prev_stride, float decay,
+                      float* out, int64_t out_stride, void* stream);
+
+/* keep[h][0 .. budget - 1]: per kv head the positions to keep of 0 .. len - 1, ascending: the first `sink`, the last
+ * `recent`, and of the others those of the largest weights[h][pos], of equal ones the first (NaN counts as the smallest).
+ * sink + recent <= budget <= len. weights_out: the kept keys' weights [kv_heads][out_stride], or NULL. */
+int lfm3a_evict_select(const float* weights, int64_t stride, int kv_heads, int len, int sink, int recent, int budget,
+                       int32_t* keep, float* weights_out, int64_t out_stride, void* stream);
+
+/* Moves the kept tokens (keep as above, of a sequence of len tokens, `sealed` of them sealed) of src into dst, token i of
+ * head h from position keep[h][i]: blocks are sealed anew from the values (code * scale), an incomplete last block goes
+ * to dst's tail in fp16, so dst holds budget tokens, budget / 32 * 32 of them sealed. dst: a view of the same layout
+ * whose blocks are not src's and whose tail is another. */
+int lfm3a_kv8_compact(const lfm3a_kv8_view* src, int len, int sealed, const int32_t* keep, int budget,
+                      const lfm3a_kv8_view* dst, void* stream);
 
 /* ---------------------------------------------------------------- test hooks */
 /* The u8 quantiser of softmax rows in the reference's operation order (kernels/prefill_attn.hip:305-331):

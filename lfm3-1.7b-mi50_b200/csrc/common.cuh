@@ -11,6 +11,7 @@
 namespace lfm3a {
 
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kBlockTokens = 32;   // KV block (engine.go:31)
 constexpr int kQuantBlock = 64;    // int8 V block and prefill key tile
 constexpr float kLazy = 8.f;       // prefill_attn.hip:33: rescale only when a tile beats the max by 2^8
@@ -250,6 +251,18 @@ __device__ __forceinline__ float max64(const float (&x)[64]) {
     for (int i = 0; i < 4; ++i) m[i] = fmax3(m[i], x[k + i], x[k + 4 + i]);
 #pragma unroll
   for (int i = 0; i < 4; ++i) m[i] = fmaxf(m[i], x[60 + i]);
+  return fmaxf(fmax3(m[0], m[1], m[2]), m[3]);
+}
+
+// Maximum of 32 values in the same way.
+__device__ __forceinline__ float max32(const float* x) {
+  float m[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+  for (int k = 4; k < 28; k += 8)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m[i] = fmax3(m[i], x[k + i], x[k + 4 + i]);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m[i] = fmaxf(m[i], x[28 + i]);
   return fmaxf(fmax3(m[0], m[1], m[2]), m[3]);
 }
 

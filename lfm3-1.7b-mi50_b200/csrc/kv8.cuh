@@ -1,0 +1,956 @@
+// The 8-bit KV cache with a scale per block of 32 tokens and kv head (LFM3A_MODE_I8BLK: int8, LFM3A_MODE_E4M3BLK: fp8
+// e4m3): append and sealing, reading back, attention, prefill staging and per-key attention weights.
+//
+// A page is one block. Pages that are complete and committed are sealed: x is held as q = round8(x / s), with
+// s = absmax / 127 (448 for e4m3; 1 for a block of zeros) over the page's 32 x D values of the head, K and V each.
+// The last tokens (an incomplete page, drafts that may be rolled back) stay in fp16 in a ring of 128 tokens per layer,
+// the tail, so a sealed page depends on committed tokens alone and a rollback needs no device work.
+//
+// Section of one (page, kv head), 32 + 64 D bytes: f32 K scale, f32 V scale, 24 zero bytes, K (32 D bytes), V (32 D).
+// K and V lie in the order in which the lanes of a warp (g = lane / 4, c = lane % 4) take them as the A operands of
+// mma.m16n8k16: S^T = K Q^T over 16 keys x 8 query rows, and O^T = V^T P over 16 dims x 8 rows. A dot over dims does
+// not care which dim sits at which k, so a lane takes 16 contiguous dims of a key in one 16-byte load:
+//   K byte (key, dim): chunk ((key / 16 * 2 + key / 8 % 2) * (D / 64) + dim / 64) * 32 + (key % 8) * 4 + dim / 16 % 4,
+//                      byte dim % 16
+//   V byte (key, dim): chunk (key / 16 * (D / 32) + dim / 32) * 32 + (dim % 8) * 4 + key % 8 / 2,
+//                      byte dim / 16 % 2 * 8 + dim / 8 % 2 * 4 + key / 8 % 2 * 2 + key % 2
+// so every shared-memory load of a fragment is 32 consecutive 16-byte chunks, without bank conflicts.
+#pragma once
+#include "common.cuh"
+#include "i8rec.cuh"
+#include "kv.cuh"
+#include "verify.cuh"
+
+namespace lfm3a {
+
+constexpr int kTailTokens = 128;   // tokens of the fp16 tail ring (slot = position mod 128)
+
+template <int D>
+struct Q8Section {
+  static constexpr int kHeader = 32;
+  static constexpr int kOffK = kHeader, kOffV = kHeader + 32 * D, kBytes = kHeader + 64 * D;
+  __host__ __device__ __forceinline__ static constexpr int k_chunk(int key, int dim) {
+    return (((key >> 4) * 2 + ((key >> 3) & 1)) * (D / 64) + (dim >> 6)) * 32 + (key & 7) * 4 + ((dim >> 4) & 3);
+  }
+  __host__ __device__ __forceinline__ static constexpr int v_index(int key, int dim) {
+    return (((key >> 4) * (D / 32) + (dim >> 5)) * 32 + (dim & 7) * 4 + ((key & 7) >> 1)) * 16 + ((dim >> 4) & 1) * 8 +
+           ((dim >> 3) & 1) * 4 + ((key >> 3) & 1) * 2 + (key & 1);
+  }
+};
+
+// The tail: K [kv_heads][128 slots][D], then V transposed, [kv_heads][D][128 slots] (pairs of keys in one word).
+struct TailView {
+  __half* k;
+  __half* v;
+};
+__host__ __device__ __forceinline__ TailView tail_of(__half* tail, int kv_heads, int h, int D) {
+  TailView t;
+  t.k = tail + (int64_t)h * kTailTokens * D;
+  t.v = tail + (int64_t)(kv_heads + h) * kTailTokens * D;
+  return t;
+}
+
+// fp16 values of the cache are finite: NaN becomes 0, an infinity the largest finite value of its sign.
+__device__ __forceinline__ float finite_f16(float x) { return x != x ? 0.f : fminf(fmaxf(x, -65504.f), 65504.f); }
+
+// The 8-bit code of x / scale and the value a code stands for (before the scale).
+template <bool E4M3>
+__device__ __forceinline__ uint32_t encode8(float x, float scale) {
+  const float y = __fdiv_rn(x, scale);
+  if (E4M3) {   // round to nearest even, saturating at 448
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(0.f), "f"(y));
+    return (uint32_t)r & 0xffu;
+  }
+  return (uint32_t)__float2int_rn(fminf(fmaxf(y, -127.f), 127.f)) & 0xffu;
+}
+
+// Bytes 0, 1 (LO) or 2, 3 of a word of codes as an fp16 pair. int8: 0x64NN is 1024 + NN with NN = v ^ 0x80, minus
+// 1152. e4m3: sign and the 7 other bits moved to an fp16's sign and bits 13..7, which is the value times 2^-8 (the
+// exponent bias differs by 8; subnormals come out right), so the caller's scale carries the 2^8. Both are exact.
+template <bool E4M3, bool HI>
+__device__ __forceinline__ uint32_t decode_pair(uint32_t w) {
+  if (E4M3) {
+    const uint32_t h = __byte_perm(w, 0u, HI ? 0x3424 : 0x1404);
+    return (h & 0x80008000u) | ((h >> 1) & 0x3f803f80u);
+  }
+  const uint32_t y = __byte_perm(w ^ 0x80808080u, 0x64u, HI ? 0x4342 : 0x4140);
+  __half2 v = *reinterpret_cast<const __half2*>(&y);
+  v = __hsub2(v, __floats2half2_rn(1152.f, 1152.f));
+  return *reinterpret_cast<uint32_t*>(&v);
+}
+template <bool E4M3>
+constexpr float kCodeUnit = E4M3 ? 256.f : 1.f;   // what decode_pair leaves to the scale
+
+// One code's value as fp32 (before the scale).
+template <bool E4M3>
+__device__ __forceinline__ float decode8(uint32_t byte) {
+  const float2 f = unpack_half2(decode_pair<E4M3, false>(byte));
+  return f.x * kCodeUnit<E4M3>;
+}
+
+__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+// ---------------------------------------------------------------- append and sealing
+// Seals one page and kv head from fp32 rows in shared memory (x [2][32][D + 1]: K, then V; the odd row stride keeps the
+// V chunks' walk over dims free of bank conflicts), by 256 threads.
+constexpr int kSealThreads = 256;
+template <int D>
+constexpr int kSealRow = D + 1;
+template <int D, bool E4M3>
+__device__ __forceinline__ void seal_page(const float* x, float* red, char* sec) {
+  using S = Q8Section<D>;
+  constexpr int RS = kSealRow<D>;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  float scale[2];
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    const float* xs = x + s * 32 * RS;
+    float amax = 0.f;
+    for (int i = tid; i < 32 * D; i += kSealThreads) amax = fmaxf(amax, fabsf(xs[(i / D) * RS + i % D]));
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    if (lane == 0) red[8 * s + warp] = amax;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    float amax = red[8 * s];
+#pragma unroll
+    for (int w = 1; w < 8; ++w) amax = fmaxf(amax, red[8 * s + w]);
+    scale[s] = amax > 0.f ? __fdiv_rn(amax, E4M3 ? 448.f : 127.f) : 1.f;
+  }
+  if (tid < 8) reinterpret_cast<float*>(sec)[tid] = tid < 2 ? scale[tid] : 0.f;
+  uint4* K = reinterpret_cast<uint4*>(sec + S::kOffK);
+  uint4* V = reinterpret_cast<uint4*>(sec + S::kOffV);
+  for (int i = tid; i < 2 * D; i += kSealThreads) {   // 16-byte chunks of K: 16 dims of one key
+    const int l = i & 31, a = i >> 5;
+    const int key = (a / (D / 64)) * 8 + (l >> 2), dim0 = (a % (D / 64)) * 64 + (l & 3) * 16;
+    uint32_t w[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      w[k] = 0;
+#pragma unroll
+      for (int b = 0; b < 4; ++b) w[k] |= encode8<E4M3>(x[key * RS + dim0 + 4 * k + b], scale[0]) << (8 * b);
+    }
+    K[i] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  const float* v = x + 32 * RS;
+  for (int i = tid; i < 2 * D; i += kSealThreads) {   // of V: four dims of four keys
+    const int l = i & 31, a = i >> 5;
+    const int key0 = (a / (D / 32)) * 16 + (l & 3) * 2, dim0 = (a % (D / 32)) * 32 + (l >> 2);
+    uint32_t w[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      w[k] = 0;
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+        w[k] |= encode8<E4M3>(v[(key0 + (b & 1) + 8 * (b >> 1)) * RS + dim0 + 8 * k], scale[1]) << (8 * b);
+    }
+    V[i] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+struct Kv8AppendArgs {
+  AppendArgs a;      // pool geometry, new rows, RoPE table, k-norm, pos0, n
+  __half* tail;
+  int page0;         // first page of the launch
+  int seal_page_end; // pages below are sealed, the others go to the tail
+};
+
+// One block per (page, kv head): the page's tokens below pos0 come from the tail, the others from the new rows. Bound
+// by memory for prompt chunks, by latency for drafts; the fp16 K is the one lfm3a_kv_append stores.
+template <int D, bool E4M3>
+__global__ __launch_bounds__(kSealThreads) void kv8_append_kernel(Kv8AppendArgs args) {
+  constexpr int J = D / 64, HALF = D / 2, RS = kSealRow<D>;
+  __shared__ float x[2 * 32 * RS];
+  __shared__ float red[16];
+  pdl_wait();
+  pdl_trigger();
+  const AppendArgs& a = args.a;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int page = args.page0 + blockIdx.x, h = blockIdx.y, t0 = page * kBlockTokens;
+  const int end = min(t0 + kBlockTokens, a.pos0 + a.n);
+  const bool sealing = page < args.seal_page_end;
+  const TailView tail = tail_of(args.tail, a.g.kv_heads, h, D);
+  if (sealing) {
+    const int old = min(a.pos0, t0 + kBlockTokens) - t0;   // tokens that wait in the tail
+    for (int i = tid; i < old * D; i += kSealThreads) {
+      const int t = i / D, d = i % D;
+      x[t * RS + d] = __half2float(tail.k[(int64_t)((t0 + t) % kTailTokens) * D + d]);
+    }
+    for (int i = tid; i < kBlockTokens * D; i += kSealThreads) {
+      const int t = i & 31, d = i >> 5;
+      if (t < old) x[32 * RS + t * RS + d] = __half2float(tail.v[d * kTailTokens + (t0 + t) % kTailTokens]);
+    }
+  }
+  for (int t = max(t0, a.pos0) + warp; t < end; t += 8) {
+    const int i = t - a.pos0, r = t - t0, slot = t % kTailTokens;
+    const __half* ks = a.k + (int64_t)i * a.stride + h * D;
+    const __half* vs = a.v + (int64_t)i * a.stride + h * D;
+    float ra[J], rb[J];
+    norm_rope_pairs<D>(a, ks, t, lane, ra, rb);
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const int d0 = lane + 32 * j, d1 = d0 + HALF;
+      const float k0 = finite_f16(ra[j]), k1 = finite_f16(rb[j]);
+      const float v0 = finite_f16(__half2float(vs[d0])), v1 = finite_f16(__half2float(vs[d1]));
+      if (sealing) {
+        x[r * RS + d0] = k0;
+        x[r * RS + d1] = k1;
+        x[32 * RS + r * RS + d0] = v0;
+        x[32 * RS + r * RS + d1] = v1;
+      } else {
+        tail.k[(int64_t)slot * D + d0] = __float2half_rn(k0);
+        tail.k[(int64_t)slot * D + d1] = __float2half_rn(k1);
+        tail.v[d0 * kTailTokens + slot] = __float2half_rn(v0);
+        tail.v[d1 * kTailTokens + slot] = __float2half_rn(v1);
+      }
+    }
+  }
+  if (!sealing) return;
+  __syncthreads();
+  seal_page<D, E4M3>(x, red, a.g.pool + phys_block(a.g, page) * a.g.block_bytes + h * a.g.head_bytes);
+}
+
+// ---------------------------------------------------------------- reading back
+struct Kv8ReadArgs {
+  KvGeom g;
+  __half* tail;
+  __half* k;       // [n][kv_heads][D]
+  __half* v;
+  int pos0, n, sealed;
+};
+
+// One block per (page, kv head): the values the cache stands for, rounded to fp16.
+template <int D, bool E4M3>
+__global__ __launch_bounds__(256) void kv8_read_kernel(Kv8ReadArgs a) {
+  using S = Q8Section<D>;
+  pdl_wait();
+  pdl_trigger();
+  const int tid = threadIdx.x, page = a.pos0 / kBlockTokens + blockIdx.x, h = blockIdx.y, t0 = page * kBlockTokens;
+  const int lo = max(a.pos0, t0), hi = min(a.pos0 + a.n, t0 + kBlockTokens);
+  const int64_t row = (int64_t)a.g.kv_heads * D;
+  if (t0 < a.sealed) {
+    const char* sec = a.g.pool + phys_block(a.g, page) * a.g.block_bytes + h * a.g.head_bytes;
+    const float ks = reinterpret_cast<const float*>(sec)[0], vs = reinterpret_cast<const float*>(sec)[1];
+    for (int i = tid; i < 32 * (D / 2); i += 256) {   // pairs of dims
+      const int t = i / (D / 2), d = 2 * (i % (D / 2));
+      if (t0 + t < lo || t0 + t >= hi) continue;
+      const int64_t at = (t0 + t - a.pos0) * row + h * D + d;
+      const uint32_t kk = *reinterpret_cast<const uint16_t*>(sec + S::kOffK + S::k_chunk(t, d) * 16 + (d & 15));
+      const uint32_t v0 = (uint8_t)sec[S::kOffV + S::v_index(t, d)], v1 = (uint8_t)sec[S::kOffV + S::v_index(t, d + 1)];
+      const float2 kf = unpack_half2(decode_pair<E4M3, false>(kk));
+      *reinterpret_cast<uint32_t*>(a.k + at) =
+          pack_half2(kf.x * kCodeUnit<E4M3> * ks, kf.y * kCodeUnit<E4M3> * ks);
+      *reinterpret_cast<uint32_t*>(a.v + at) = pack_half2(decode8<E4M3>(v0) * vs, decode8<E4M3>(v1) * vs);
+    }
+  } else {
+    const TailView tail = tail_of(a.tail, a.g.kv_heads, h, D);
+    for (int i = tid; i < 32 * D; i += 256) {
+      const int t = t0 + i / D, d = i % D, slot = t % kTailTokens;
+      if (t < lo || t >= hi) continue;
+      const int64_t at = (t - a.pos0) * row + h * D + d;
+      a.k[at] = tail.k[(int64_t)slot * D + d];
+      a.v[at] = tail.v[d * kTailTokens + slot];
+    }
+  }
+}
+
+// ---------------------------------------------------------------- attention
+struct Kv8AttnArgs {
+  KvGeom g;
+  __half* tail;
+  const __half* q;      // row (t, qh) at q + t * q_stride + qh * D
+  const __half* gate;   // [m][q_heads] logits, or null
+  __half* out;          // [m][q_heads][D] (one split)
+  float* lse;           // [m][q_heads] natural-log sum of exponentials, or null
+  float* part;          // [m * q_heads][splits][D + 2] (several splits)
+  int64_t q_stride;
+  int m, group, q_heads, ctx_len, window, sealed, splits;
+  int p_begin, p_total; // pages of [start, ctx_len + m)
+  float qk_scale;       // (1 / sqrt(D)) log2(e)
+};
+
+// The query rows of one kv head as B operands (r = t * group + j): chunk ((n-tile * D / 64 + e) * 2 + s) * 32 + lane
+// holds dims 64 e + 16 c + 8 s .. + 7 of row 8 n-tile + g: b0, b1 of k-steps 2 s and 2 s + 1. Rows past m * group are 0.
+template <int D>
+__device__ __forceinline__ void stage_q(const __half* q, int64_t q_stride, int rows, int group, int h, int row0, int ntiles,
+                                        uint4* sq, int tid, int threads) {
+  for (int i = tid; i < ntiles * D; i += threads) {
+    const int l = i & 31, k = i >> 5, s = k & 1, e = (k >> 1) % (D / 64), nt = (k >> 1) / (D / 64);
+    const int r = row0 + 8 * nt + (l >> 2);
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (r < rows) {
+      const int t = r / group, j = r - t * group;
+      v = *reinterpret_cast<const uint4*>(q + t * q_stride + (int64_t)(h * group + j) * D + 64 * e + 16 * (l & 3) + 8 * s);
+    }
+    sq[i] = v;
+  }
+}
+
+// Whether every row sees every key of the page (rows at ctx_len .. ctx_len + m - 1).
+__device__ __forceinline__ bool page_open(int page, int ctx_len, int m, int window) {
+  return page * kBlockTokens + kBlockTokens - 1 <= ctx_len &&
+         (window == 0 || page * kBlockTokens > ctx_len + m - 1 - window);
+}
+__device__ __forceinline__ bool sees(int pos, int key, int window) {
+  return key <= pos && (window == 0 || key > pos - window);
+}
+
+template <int D, int NT>
+struct Kv8Attn {
+  // 32 rows at head_dim 64 need about 160 registers: 12 warps in one block per SM; else 8 warps, two blocks per SM at
+  // head_dim 64 (ring and registers allow it), one at 128.
+  static constexpr bool kWide = D == 64 && NT == 4;
+  static constexpr int kWarps = kWide ? 12 : 8, kThreads = 32 * kWarps, kStages = kWide ? 4 : 3;
+  static constexpr int kStageBytes = Q8Section<D>::kBytes;                 // a multiple of 32
+  static constexpr int kRing = kWarps * kStages * kStageBytes;
+  static constexpr int kOStride = D + 4;                                   // floats, 4 mod 32 banks
+  static constexpr int kMerge = kWarps * 8 * NT * (kOStride + 2) * 4;      // over the ring once it is drained
+  static constexpr int kOffQ = kRing > kMerge ? kRing : kMerge;
+  static constexpr int kOffBar = kOffQ + 8 * NT * D * 2;
+  static constexpr int kSmem = kOffBar + kWarps * kStages * 8;
+  static constexpr int kBlocksPerSm = D == 64 && !kWide ? 2 : 1;
+};
+
+// Fragments of a tail page straight from the ring in global memory (fp16, L2-resident).
+template <int D>
+__device__ __forceinline__ void tail_k_frag(const TailView& t, int key0, int e, int g, int c, uint2 (&kA)[4],
+                                            uint2 (&kB)[4]) {
+  const uint4* a = reinterpret_cast<const uint4*>(t.k + (int64_t)((key0 + g) % kTailTokens) * D + 64 * e + 16 * c);
+  const uint4* b = reinterpret_cast<const uint4*>(t.k + (int64_t)((key0 + g + 8) % kTailTokens) * D + 64 * e + 16 * c);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint4 x = a[i], y = b[i];
+    kA[2 * i] = make_uint2(x.x, x.y);
+    kA[2 * i + 1] = make_uint2(x.z, x.w);
+    kB[2 * i] = make_uint2(y.x, y.y);
+    kB[2 * i + 1] = make_uint2(y.z, y.w);
+  }
+}
+// The pair of keys key, key + 1 (key even) at one dim, 0 past the sequence's end: a stale slot may hold anything.
+__device__ __forceinline__ uint32_t tail_v_pair(const TailView& t, int key, int dim, int kv_end) {
+  uint32_t w = *reinterpret_cast<const uint32_t*>(t.v + (int64_t)dim * kTailTokens + key % kTailTokens);
+  if (key + 1 >= kv_end) w &= key >= kv_end ? 0u : 0xffffu;
+  return w;
+}
+
+// Attention of up to 8 NT query rows of one kv head over a split's pages. Grid (splits, kv heads, row groups).
+//
+// Each warp streams its own pages (every 8th of the split's) through its own ring of bulk copies, so no warp waits for
+// another before the end, and turns codes into fp16 operands in registers: Q, K and P V products are exact to fp32
+// accumulation, only P is rounded to fp16. Scores come as S^T (keys x rows), so the sealed pages' K scale is one factor
+// per page, and the V scale is folded into the exponent: P' = 2^(s + log2 vs - m'), with m' the running maximum of
+// s + log2 vs, gives sum P' v8 = 2^-m' sum 2^s v directly, and l = sum P' / vs is the softmax sum. m' is lazy (moved
+// only when a score passes it by 2^8; fp16 P then stays below 2^8 and fp32 sums are unaffected), so the common page
+// needs no shuffles but one vote. movmatrix turns the S^T accumulators into the B operand of O^T = V^T P.
+// The warps meet in shared memory at the end; one split writes its rows, several write (acc, m', l) partials.
+template <int D, int NT, bool E4M3>
+__global__ __launch_bounds__(Kv8Attn<D, NT>::kThreads, Kv8Attn<D, NT>::kBlocksPerSm) void kv8_attend_kernel(Kv8AttnArgs a) {
+  using L = Kv8Attn<D, NT>;
+  using S = Q8Section<D>;
+  constexpr int NE = D / 64, W = L::kWarps, NS = L::kStages, NR = 8 * NT;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  const int h = blockIdx.y, split = blockIdx.x, row0 = blockIdx.z * NR, rows = a.m * a.group;
+  const int kv_end = a.ctx_len + a.m;
+  const int pg0 = a.p_begin + (int)((int64_t)a.p_total * split / a.splits);
+  const int pg1 = a.p_begin + (int)((int64_t)a.p_total * (split + 1) / a.splits);
+  const int sealed_pages = a.sealed / kBlockTokens;
+  uint4* sq = reinterpret_cast<uint4*>(smem + L::kOffQ);
+  uint8_t* ring = smem + (size_t)warp * NS * L::kStageBytes;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kOffBar) + warp * NS;
+
+  if (lane == 0) {
+    for (int s = 0; s < NS; ++s) mbar_init(&full[s], 1);
+    fence_barrier_init();
+  }
+  __syncwarp();
+  pdl_wait();
+  const char* head = a.g.pool + h * a.g.head_bytes;
+  auto issue = [&](int page, int st) {
+    mbar_arrive_expect_tx(&full[st], L::kStageBytes);
+    bulk_g2s(ring + st * L::kStageBytes, head + phys_block(a.g, page) * a.g.block_bytes, L::kStageBytes, &full[st]);
+  };
+  const int first = pg0 + warp;
+  int issued = 0, waited = 0;
+  if (lane == 0)
+    for (int p = first; issued < NS && p < pg1 && p < sealed_pages; p += W) issue(p, issued++);
+  issued = __shfl_sync(0xffffffffu, issued, 0);
+  stage_q<D>(a.q, a.q_stride, rows, a.group, h, row0, NT, sq, threadIdx.x, L::kThreads);
+  __syncthreads();
+
+  float o[D / 16][NT][4];
+  float mr[NT][2];
+  float lr[NT][2], lp[NT][2];   // sums of P' / vs, exact and with P' as rounded to fp16
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      mr[n][i] = -INFINITY;
+      lr[n][i] = lp[n][i] = 0.f;
+    }
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[d][n][i] = 0.f;
+  }
+
+  const TailView tail = tail_of(a.tail, a.g.kv_heads, h, D);
+  // Softmax of 16 keys (S^T in s) against this warp's rows, P' packed as B operands. kc: the scores' factor, lv: log2 of
+  // the V scale, inv: its reciprocal.
+  auto softmax16 = [&](float (&s)[NT][4], int key0, bool open, float kc, float lv, float inv, uint32_t (&pb)[NT][2]) {
+    if (!open) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int pos = a.ctx_len + (row0 + 8 * n + 2 * c + (i & 1)) / a.group;
+          if (!sees(pos, key0 + g + 8 * (i >> 1), a.window)) s[n][i] = -INFINITY;   // kc > 0 keeps it
+        }
+    }
+    float x[NT][4];
+    float top = -INFINITY;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[n][i] = fmaf(s[n][i], kc, lv - mr[n][i & 1]);
+      // a masked score against a row without a maximum yet is -inf + inf: it stays masked
+      if (!open) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[n][i] = s[n][i] == -INFINITY ? -INFINITY : x[n][i];
+      }
+      top = fmaxf(fmax3(top, x[n][0], x[n][1]), fmaxf(x[n][2], x[n][3]));
+    }
+    if (__any_sync(0xffffffffu, top > kLazy)) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float mx = fmaxf(fmaf(s[n][i], kc, lv), fmaf(s[n][i + 2], kc, lv));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+          mx = fmaxf(mx, mr[n][i]);
+          const float f = mx == -INFINITY ? 1.f : fast_exp2(mr[n][i] - mx);   // no key yet: 2^-inf = 0
+          mr[n][i] = mx;
+          lr[n][i] *= f;
+          lp[n][i] *= f;
+#pragma unroll
+          for (int d = 0; d < D / 16; ++d) {
+            o[d][n][i] *= f;
+            o[d][n][i + 2] *= f;
+          }
+          const float off = lv - (mx == -INFINITY ? 0.f : mx);
+          x[n][i] = fmaf(s[n][i], kc, off);
+          x[n][i + 2] = fmaf(s[n][i + 2], kc, off);
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      float p[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p[i] = fast_exp2(x[n][i]);
+      const uint32_t h0 = pack_half2(p[0], p[1]), h1 = pack_half2(p[2], p[3]);
+      const float2 r = fadd2(unpack_half2(h0), unpack_half2(h1));
+      lr[n][0] = fmaf(p[0] + p[2], inv, lr[n][0]);
+      lr[n][1] = fmaf(p[1] + p[3], inv, lr[n][1]);
+      lp[n][0] = fmaf(r.x, inv, lp[n][0]);
+      lp[n][1] = fmaf(r.y, inv, lp[n][1]);
+      pb[n][0] = movmatrix_trans(h0);
+      pb[n][1] = movmatrix_trans(h1);
+    }
+  };
+
+  bool ok = true;
+  int st = 0, next = first + issued * W;
+  uint32_t phase = 0;
+  for (int page = first; page < pg1 && page < sealed_pages; page += W) {
+    ok = __all_sync(0xffffffffu, mbar_wait(&full[st], phase));
+    if (!ok) break;
+    ++waited;
+    const uint8_t* sec = ring + st * L::kStageBytes;
+    const float ks = reinterpret_cast<const float*>(sec)[0], vs = reinterpret_cast<const float*>(sec)[1];
+    const float kc = ks * kCodeUnit<E4M3> * a.qk_scale, vu = vs * kCodeUnit<E4M3>;
+    const float lv = __log2f(vu), inv = __fdividef(1.f, vu);
+    const bool open = page_open(page, a.ctx_len, a.m, a.window);
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt) {
+      float s[NT][4];
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[n][i] = 0.f;
+      const uint4* kc4 = reinterpret_cast<const uint4*>(sec + S::kOffK) + (mt * 2 * NE) * 32 + lane;
+#pragma unroll
+      for (int e = 0; e < NE; ++e) {
+        const uint4 ra = kc4[e * 32], rb = kc4[(NE + e) * 32];
+        const uint32_t wa[4] = {ra.x, ra.y, ra.z, ra.w}, wb[4] = {rb.x, rb.y, rb.z, rb.w};
+#pragma unroll
+        for (int s2 = 0; s2 < 2; ++s2) {
+          uint32_t fa[2][4];
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            fa[u][0] = decode_pair<E4M3, false>(wa[2 * s2 + u]);
+            fa[u][1] = decode_pair<E4M3, false>(wb[2 * s2 + u]);
+            fa[u][2] = decode_pair<E4M3, true>(wa[2 * s2 + u]);
+            fa[u][3] = decode_pair<E4M3, true>(wb[2 * s2 + u]);
+          }
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            const uint4 qv = sq[((n * NE + e) * 2 + s2) * 32 + lane];
+            mma_f16_16816(s[n], fa[0], qv.x, qv.y);
+            mma_f16_16816(s[n], fa[1], qv.z, qv.w);
+          }
+        }
+      }
+      uint32_t pb[NT][2];
+      softmax16(s, page * kBlockTokens + 16 * mt, open, kc, lv, inv, pb);
+      const uint4* vc4 = reinterpret_cast<const uint4*>(sec + S::kOffV) + mt * (D / 32) * 32 + lane;
+#pragma unroll
+      for (int d = 0; d < D / 32; ++d) {
+        const uint4 r = vc4[d * 32];
+        const uint32_t f0[4] = {decode_pair<E4M3, false>(r.x), decode_pair<E4M3, false>(r.y),
+                                decode_pair<E4M3, true>(r.x), decode_pair<E4M3, true>(r.y)};
+        const uint32_t f1[4] = {decode_pair<E4M3, false>(r.z), decode_pair<E4M3, false>(r.w),
+                                decode_pair<E4M3, true>(r.z), decode_pair<E4M3, true>(r.w)};
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          mma_f16_16816(o[2 * d][n], f0, pb[n][0], pb[n][1]);
+          mma_f16_16816(o[2 * d + 1][n], f1, pb[n][0], pb[n][1]);
+        }
+      }
+    }
+    __syncwarp();   // every lane has read the stage
+    if (next < pg1 && next < sealed_pages) {
+      if (lane == 0) issue(next, st);
+      ++issued;
+    }
+    next += W;
+    if (++st == NS) {
+      st = 0;
+      phase ^= 1;
+    }
+  }
+  if (!ok) {   // give up: raise the error word and drain this warp's own copies (bounded)
+    if (lane == 0) raise_error(kErrWaitFull);
+    for (; waited < issued; ++waited) {
+      (void)mbar_wait(&full[st], phase);
+      if (++st == NS) {
+        st = 0;
+        phase ^= 1;
+      }
+    }
+  }
+  // Tail pages (fp16): the first one of this warp's at or past the sealed ones.
+  int page = first;
+  if (page < sealed_pages) page += (sealed_pages - page + W - 1) / W * W;
+  for (; page < pg1; page += W) {
+#pragma unroll 1
+    for (int mt = 0; mt < 2; ++mt) {
+      const int key0 = page * kBlockTokens + 16 * mt;
+      if (key0 >= kv_end) break;
+      float s[NT][4];
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[n][i] = 0.f;
+#pragma unroll
+      for (int e = 0; e < NE; ++e) {
+        uint2 kA[4], kB[4];
+        tail_k_frag<D>(tail, key0, e, g, c, kA, kB);
+#pragma unroll
+        for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            const uint4 qv = sq[((n * NE + e) * 2 + s2) * 32 + lane];
+            const uint32_t f0[4] = {kA[2 * s2].x, kB[2 * s2].x, kA[2 * s2].y, kB[2 * s2].y};
+            const uint32_t f1[4] = {kA[2 * s2 + 1].x, kB[2 * s2 + 1].x, kA[2 * s2 + 1].y, kB[2 * s2 + 1].y};
+            mma_f16_16816(s[n], f0, qv.x, qv.y);
+            mma_f16_16816(s[n], f1, qv.z, qv.w);
+          }
+      }
+      uint32_t pb[NT][2];
+      softmax16(s, key0, false, a.qk_scale, 0.f, 1.f, pb);
+      const int k0 = key0 + 2 * c;
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) {
+        const int dim = 16 * d + g;
+        const uint32_t f[4] = {tail_v_pair(tail, k0, dim, kv_end), tail_v_pair(tail, k0, dim + 8, kv_end),
+                               tail_v_pair(tail, k0 + 8, dim, kv_end), tail_v_pair(tail, k0 + 8, dim + 8, kv_end)};
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma_f16_16816(o[d][n], f, pb[n][0], pb[n][1]);
+      }
+    }
+  }
+
+  // The warps' rows meet in shared memory: [warp][row][D + 4] acc, then [warp][row] (max, sum).
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+      for (int x = 4; x <= 16; x <<= 1) {
+        lr[n][i] += __shfl_xor_sync(0xffffffffu, lr[n][i], x);
+        lp[n][i] += __shfl_xor_sync(0xffffffffu, lp[n][i], x);
+      }
+      // acc / lp is the mean over P' as rounded (numerator and denominator carry the same roundings); from here on
+      // acc is relative to the exact sum, which the log-sum-exp needs
+      const float f = lp[n][i] > 0.f ? lr[n][i] / lp[n][i] : 1.f;
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) {
+        o[d][n][i] *= f;
+        o[d][n][i + 2] *= f;
+      }
+    }
+  __syncthreads();   // the rings are drained
+  float* so = reinterpret_cast<float*>(smem);
+  float2* sm = reinterpret_cast<float2*>(smem + W * NR * L::kOStride * 4);
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = 8 * n + 2 * c + i;
+      float* dst = so + (warp * NR + r) * L::kOStride + g;
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) {
+        dst[16 * d] = o[d][n][i];
+        dst[16 * d + 8] = o[d][n][i + 2];
+      }
+      if (g == 0) sm[warp * NR + r] = make_float2(mr[n][i], lr[n][i]);
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < NR * (D / 2); i += L::kThreads) {
+    const int r = i / (D / 2), d = 2 * (i % (D / 2)), gr = row0 + r;
+    if (gr >= rows) break;
+    float2 ml[W];
+    float mx = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      ml[w] = sm[w * NR + r];
+      mx = fmaxf(mx, ml[w].x);
+    }
+    float l = 0.f, x0 = 0.f, x1 = 0.f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const float f = ml[w].x == -INFINITY ? 0.f : fast_exp2(ml[w].x - mx);
+      const float2 v = *reinterpret_cast<const float2*>(so + (w * NR + r) * L::kOStride + d);
+      l = fmaf(f, ml[w].y, l);
+      x0 = fmaf(f, v.x, x0);
+      x1 = fmaf(f, v.y, x1);
+    }
+    const int t = gr / a.group, row = t * a.q_heads + h * a.group + (gr - t * a.group);
+    if (a.splits == 1) {
+      const float scale = (l > 0.f ? 1.f / l : 0.f) * sigmoid_gate(a.gate, row);
+      *reinterpret_cast<uint32_t*>(a.out + (int64_t)row * D + d) = pack_half2(x0 * scale, x1 * scale);
+      if (a.lse && d == 0) a.lse[row] = (mx + log2f(l)) * kLn2;
+    } else {
+      float* dst = a.part + ((int64_t)row * a.splits + split) * (D + 2);
+      *reinterpret_cast<float2*>(dst + d) = make_float2(x0, x1);
+      if (d == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(mx, l);
+    }
+  }
+}
+
+// Merge of a row's split partials (acc[D], max, sum): one block of 128 threads per row, thread = (pair of dims, group
+// of splits), each thread's loads independent; the weights 2^(m - M) in shared memory.
+constexpr int kKv8CombineThreads = 128, kKv8MaxSplits = 1024;
+template <int D>
+__global__ __launch_bounds__(kKv8CombineThreads) void kv8_combine_kernel(const float* part, int splits, const __half* gate,
+                                                                         __half* out, float* lse) {
+  constexpr int P = D / 2, G = kKv8CombineThreads / P;
+  __shared__ float w[kKv8MaxSplits];
+  __shared__ float red[32];
+  __shared__ float2 acc[G][P];
+  pdl_wait();
+  pdl_trigger();
+  const int row = blockIdx.x, tid = threadIdx.x, p = tid % P, gi = tid / P;
+  const float* base = part + (int64_t)row * splits * (D + 2);
+  float mx = -INFINITY;
+  for (int s = tid; s < splits; s += kKv8CombineThreads) {
+    w[s] = base[(int64_t)s * (D + 2) + D];
+    mx = fmaxf(mx, w[s]);
+  }
+  mx = block_reduce(mx, true, red);
+  float l = 0.f;
+  for (int s = tid; s < splits; s += kKv8CombineThreads) {
+    const float f = w[s] == -INFINITY ? 0.f : fast_exp2(w[s] - mx);
+    l = fmaf(f, base[(int64_t)s * (D + 2) + D + 1], l);
+    w[s] = f;
+  }
+  l = block_reduce(l, false, red);   // its barriers also publish w
+  float2 x = make_float2(0.f, 0.f);
+#pragma unroll 8
+  for (int s = gi; s < splits; s += G) {
+    const float2 v = *reinterpret_cast<const float2*>(base + (int64_t)s * (D + 2) + 2 * p);
+    x.x = fmaf(w[s], v.x, x.x);
+    x.y = fmaf(w[s], v.y, x.y);
+  }
+  acc[gi][p] = x;
+  __syncthreads();
+  if (gi == 0) {
+#pragma unroll
+    for (int k = 1; k < G; ++k) {
+      x.x += acc[k][p].x;
+      x.y += acc[k][p].y;
+    }
+    const float scale = (l > 0.f ? 1.f / l : 0.f) * sigmoid_gate(gate, row);
+    *reinterpret_cast<uint32_t*>(out + (int64_t)row * D + 2 * p) = pack_half2(x.x * scale, x.y * scale);
+    if (lse && p == 0) lse[row] = (mx + log2f(l)) * kLn2;
+  }
+}
+
+// ---------------------------------------------------------------- prefill staging
+template <int D>
+constexpr int kStagedHeadBytes = F16Section<D>::kOffV8;   // a MODE_F16 section without the int8 V copy: K, then V
+
+struct Kv8ExpandArgs {
+  KvGeom g;
+  __half* tail;
+  char* dst;         // staged sections [page][kv head]
+  int32_t* table;    // the staged pages' block table, logical pages page0 .. page0 + grid.x - 1
+  float4* scales;    // [page - page0][kv head]: K factor, log2 of the V factor, its reciprocal
+  int page0, sealed, len;
+};
+
+// One page and kv head of the cache as the K and V tiles of a MODE_F16 section, the codes as fp16 (exactly; the scales go
+// beside them): what the prefill kernel's SCALED form reads. Values past the sequence's end are 0.
+template <int D, bool E4M3>
+__global__ __launch_bounds__(256) void kv8_expand_kernel(Kv8ExpandArgs a) {
+  using S = Q8Section<D>;
+  using F = F16Section<D>;
+  pdl_wait();
+  pdl_trigger();
+  const int tid = threadIdx.x, page = a.page0 + blockIdx.x, h = blockIdx.y, t0 = page * kBlockTokens;
+  if (h == 0 && tid == 0) a.table[page] = blockIdx.x;
+  const int64_t section = (int64_t)blockIdx.x * a.g.kv_heads + h;
+  char* dst = a.dst + section * kStagedHeadBytes<D>;
+  uint4* K = reinterpret_cast<uint4*>(dst);
+  uint4* V = reinterpret_cast<uint4*>(dst + F::kOffV);
+  if (t0 < a.sealed) {
+    const char* sec = a.g.pool + phys_block(a.g, page) * a.g.block_bytes + h * a.g.head_bytes;
+    if (tid == 0) {
+      const float ks = reinterpret_cast<const float*>(sec)[0] * kCodeUnit<E4M3>;
+      const float vs = reinterpret_cast<const float*>(sec)[1] * kCodeUnit<E4M3>;
+      a.scales[section] = make_float4(ks, log2f(vs), 1.f / vs, 0.f);
+    }
+    for (int i = tid; i < 4 * D; i += 256) {   // 16-byte rows of the tiles: 8 dims of one key, 8 keys of one dim
+      const int e = i & 7, tile = i >> 3;
+      const int key = (tile / (D / 8)) * 8 + e, d = (tile % (D / 8)) * 8;
+      const uint2 w = *reinterpret_cast<const uint2*>(sec + S::kOffK + S::k_chunk(key, d) * 16 + (d & 15));
+      K[i] = make_uint4(decode_pair<E4M3, false>(w.x), decode_pair<E4M3, true>(w.x), decode_pair<E4M3, false>(w.y),
+                        decode_pair<E4M3, true>(w.y));
+      const int vd = (tile >> 2) * 8 + e, key0 = (tile & 3) * 8;
+      uint32_t v[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)   // keys key0 + 2 k and the next lie in neighbouring bytes
+        v[k] = decode_pair<E4M3, false>(
+            *reinterpret_cast<const uint16_t*>(sec + S::kOffV + S::v_index(key0 + 2 * k, vd)));
+      V[i] = make_uint4(v[0], v[1], v[2], v[3]);
+    }
+    return;
+  }
+  const TailView tail = tail_of(a.tail, a.g.kv_heads, h, D);
+  if (tid == 0) a.scales[section] = make_float4(1.f, 0.f, 1.f, 0.f);
+  for (int i = tid; i < 4 * D; i += 256) {
+    const int e = i & 7, tile = i >> 3;
+    const int key = (tile / (D / 8)) * 8 + e, d = (tile % (D / 8)) * 8;
+    K[i] = t0 + key < a.len ? *reinterpret_cast<const uint4*>(tail.k + (int64_t)((t0 + key) % kTailTokens) * D + d)
+                            : make_uint4(0, 0, 0, 0);
+    const int vd = (tile >> 2) * 8 + e, key0 = (tile & 3) * 8;
+    uint32_t v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      v[k] = t0 + key0 + 2 * k < a.len ? tail_v_pair(tail, t0 + key0 + 2 * k, vd, a.len) : 0u;
+    V[i] = make_uint4(v[0], v[1], v[2], v[3]);
+  }
+}
+
+// ---------------------------------------------------------------- attention weights per key
+struct Kv8WeightArgs {
+  KvGeom g;
+  __half* tail;
+  const __half* q;
+  const float* lse;     // [m][q_heads]
+  const float* prev;    // [kv_heads][stride], or null
+  float* out;           // [kv_heads][stride]
+  int64_t q_stride, prev_stride, out_stride;
+  int m, group, q_heads, ctx_len, window, sealed, splits, pages;
+  float decay, qk_scale;
+};
+
+template <int D>
+struct Kv8Weights {
+  static constexpr int kWarps = 8, kThreads = 32 * kWarps, kStages = 4;
+  static constexpr int kStageBytes = Q8Section<D>::kOffV;   // the header and K
+  static constexpr int kRing = kWarps * kStages * kStageBytes;
+  static constexpr int kMaxRows = 256;
+  static __host__ __device__ constexpr int lse_off(int ntiles) { return kRing + ntiles * 8 * D * 2; }
+  static __host__ __device__ constexpr int bar_off(int ntiles) { return lse_off(ntiles) + ntiles * 8 * 4; }
+  static __host__ __device__ constexpr int smem(int ntiles) { return bar_off(ntiles) + kWarps * kStages * 8; }
+};
+
+// out[h][key] = decay prev[h][key] + sum over the m tokens and the head's query rows of 2^(s - lse): only K is read. A
+// warp takes a page (as kv8_attend_kernel does), makes its K operands once and passes over the query rows 8 at a time;
+// a lane owns the weights of 4 keys for 2 rows in 8, so the sums meet in two shuffles at the end and no atomics are
+// needed. Grid (splits, kv heads).
+template <int D, bool E4M3>
+__global__ __launch_bounds__(Kv8Weights<D>::kThreads, D == 64 ? 2 : 1) void kv8_weights_kernel(Kv8WeightArgs a) {
+  using L = Kv8Weights<D>;
+  using S = Q8Section<D>;
+  constexpr int NE = D / 64, W = L::kWarps, NS = L::kStages;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  const int h = blockIdx.y, rows = a.m * a.group, ntiles = (rows + 7) / 8, kv_end = a.ctx_len + a.m;
+  const int pg0 = (int)((int64_t)a.pages * blockIdx.x / a.splits), pg1 = (int)((int64_t)a.pages * (blockIdx.x + 1) / a.splits);
+  const int sealed_pages = a.sealed / kBlockTokens;
+  uint4* sq = reinterpret_cast<uint4*>(smem + L::kRing);
+  float* slse = reinterpret_cast<float*>(smem + L::lse_off(ntiles));
+  uint8_t* ring = smem + (size_t)warp * NS * L::kStageBytes;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::bar_off(ntiles)) + warp * NS;
+
+  if (lane == 0) {
+    for (int s = 0; s < NS; ++s) mbar_init(&full[s], 1);
+    fence_barrier_init();
+  }
+  __syncwarp();
+  pdl_wait();
+  const char* head = a.g.pool + h * a.g.head_bytes;
+  auto issue = [&](int page, int st) {
+    mbar_arrive_expect_tx(&full[st], L::kStageBytes);
+    bulk_g2s(ring + st * L::kStageBytes, head + phys_block(a.g, page) * a.g.block_bytes, L::kStageBytes, &full[st]);
+  };
+  const int first = pg0 + warp;
+  int issued = 0, waited = 0;
+  if (lane == 0)
+    for (int p = first; issued < NS && p < pg1 && p < sealed_pages; p += W) issue(p, issued++);
+  issued = __shfl_sync(0xffffffffu, issued, 0);
+  stage_q<D>(a.q, a.q_stride, rows, a.group, h, 0, ntiles, sq, threadIdx.x, L::kThreads);
+  for (int r = threadIdx.x; r < 8 * ntiles; r += L::kThreads) {
+    const int t = r / a.group, j = r - t * a.group;
+    // a padding row, and a row that saw no key (lse -inf), weighs nothing
+    float x = r < rows ? a.lse[t * a.q_heads + h * a.group + j] * kLog2e : INFINITY;
+    slse[r] = x == -INFINITY ? INFINITY : x;
+  }
+  __syncthreads();
+
+  const TailView tail = tail_of(a.tail, a.g.kv_heads, h, D);
+  float w[2];   // keys key0 + g, key0 + g + 8
+  auto rows16 = [&](const uint32_t (&f)[4 * NE][4], int key0, bool open, float kc) {
+    w[0] = w[1] = 0.f;
+#pragma unroll 2
+    for (int n = 0; n < ntiles; ++n) {
+      float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int e = 0; e < 2 * NE; ++e) {
+        const uint4 qv = sq[(n * 2 * NE + e) * 32 + lane];
+        mma_f16_16816(s, f[2 * e], qv.x, qv.y);
+        mma_f16_16816(s, f[2 * e + 1], qv.z, qv.w);
+      }
+      const float2 z = *reinterpret_cast<const float2*>(slse + 8 * n + 2 * c);
+      float p[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p[i] = fast_exp2(fmaf(s[i], kc, (i & 1) ? -z.y : -z.x));
+      if (!open) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int pos = a.ctx_len + (8 * n + 2 * c + (i & 1)) / a.group;
+          if (!sees(pos, key0 + g + 8 * (i >> 1), a.window)) p[i] = 0.f;
+        }
+      }
+      w[0] += p[0] + p[1];
+      w[1] += p[2] + p[3];
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      w[i] += __shfl_xor_sync(0xffffffffu, w[i], 1);
+      w[i] += __shfl_xor_sync(0xffffffffu, w[i], 2);
+      const int key = key0 + g + 8 * i;
+      if (c == 0 && key < kv_end) {
+        const float old = a.prev ? a.decay * a.prev[h * a.prev_stride + key] : 0.f;
+        a.out[h * a.out_stride + key] = old + w[i];
+      }
+    }
+  };
+
+  bool ok = true;
+  int st = 0, next = first + issued * W;
+  uint32_t phase = 0;
+  for (int page = first; page < pg1 && page < sealed_pages; page += W) {
+    ok = __all_sync(0xffffffffu, mbar_wait(&full[st], phase));
+    if (!ok) break;
+    ++waited;
+    const uint8_t* sec = ring + st * L::kStageBytes;
+    const float kc = reinterpret_cast<const float*>(sec)[0] * kCodeUnit<E4M3> * a.qk_scale;
+    const bool open = page_open(page, a.ctx_len, a.m, a.window);
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt) {
+      const uint4* kc4 = reinterpret_cast<const uint4*>(sec + S::kOffK) + (mt * 2 * NE) * 32 + lane;
+      uint32_t f[4 * NE][4];
+#pragma unroll
+      for (int e = 0; e < NE; ++e) {
+        const uint4 ra = kc4[e * 32], rb = kc4[(NE + e) * 32];
+        const uint32_t wa[4] = {ra.x, ra.y, ra.z, ra.w}, wb[4] = {rb.x, rb.y, rb.z, rb.w};
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          f[4 * e + u][0] = decode_pair<E4M3, false>(wa[u]);
+          f[4 * e + u][1] = decode_pair<E4M3, false>(wb[u]);
+          f[4 * e + u][2] = decode_pair<E4M3, true>(wa[u]);
+          f[4 * e + u][3] = decode_pair<E4M3, true>(wb[u]);
+        }
+      }
+      rows16(f, page * kBlockTokens + 16 * mt, open, kc);
+    }
+    __syncwarp();
+    if (next < pg1 && next < sealed_pages) {
+      if (lane == 0) issue(next, st);
+      ++issued;
+    }
+    next += W;
+    if (++st == NS) {
+      st = 0;
+      phase ^= 1;
+    }
+  }
+  if (!ok) {
+    if (lane == 0) raise_error(kErrWaitFull);
+    for (; waited < issued; ++waited) {
+      (void)mbar_wait(&full[st], phase);
+      if (++st == NS) {
+        st = 0;
+        phase ^= 1;
+      }
+    }
+  }
+  int page = first;
+  if (page < sealed_pages) page += (sealed_pages - page + W - 1) / W * W;
+  for (; page < pg1; page += W) {
+#pragma unroll 1
+    for (int mt = 0; mt < 2; ++mt) {
+      const int key0 = page * kBlockTokens + 16 * mt;
+      if (key0 >= kv_end) break;
+      uint32_t f[4 * NE][4];
+#pragma unroll
+      for (int e = 0; e < NE; ++e) {
+        uint2 kA[4], kB[4];
+        tail_k_frag<D>(tail, key0, e, g, c, kA, kB);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          f[4 * e + u][0] = kA[u].x;
+          f[4 * e + u][1] = kB[u].x;
+          f[4 * e + u][2] = kA[u].y;
+          f[4 * e + u][3] = kB[u].y;
+        }
+      }
+      rows16(f, key0, false, a.qk_scale);
+    }
+  }
+}
+
+}  // namespace lfm3a

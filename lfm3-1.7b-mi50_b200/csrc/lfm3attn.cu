@@ -12,9 +12,11 @@
 
 #include "../../include/lfm3attn.h"
 #include "common.cuh"
+#include "evict.cuh"
 #include "gemm.cuh"
 #include "i8rec.cuh"
 #include "kv.cuh"
+#include "kv8.cuh"
 #include "module.cuh"
 #include "pcache.h"
 #include "prefill.cuh"
@@ -85,10 +87,14 @@ int ensure_smem(K kernel, int bytes, std::atomic<bool>* done_per_device) {
   return LFM3A_OK;
 }
 
-int check_view(const lfm3a_kv_view* kv) {
+bool is_block8(int mode) { return mode == LFM3A_MODE_I8BLK || mode == LFM3A_MODE_E4M3BLK; }
+
+int check_view(const lfm3a_kv_view* kv, bool block8 = false) {
   if (!kv || !kv->pool || !kv->block_table) return fail(LFM3A_EINVAL, "null kv view, pool or block table");
   if (kv->pool_blocks <= 0) return fail(LFM3A_EINVAL, "pool_blocks must be positive");
   const lfm3a_kv_layout& L = kv->layout;
+  if (is_block8(L.mode) != block8)
+    return fail(LFM3A_ENOTSUP, "MODE_I8BLK and MODE_E4M3BLK caches go through the lfm3a_kv8_* calls, other modes do not");
   lfm3a_kv_layout want;
   const int rc = lfm3a_kv_layout_init(L.mode, L.kv_heads, L.head_dim, L.block_tokens, &want);
   if (rc != LFM3A_OK) return rc;
@@ -304,6 +310,9 @@ int lfm3a_kv_layout_init(int mode, int kv_heads, int head_dim, int block_tokens,
   } else if (mode == LFM3A_MODE_I8REC) {
     out->head_bytes = 2 * head_dim + 8;
     out->block_bytes = out->head_bytes * kv_heads * block_tokens;
+  } else if (is_block8(mode)) {
+    out->head_bytes = 32 + 64 * head_dim;
+    out->block_bytes = out->head_bytes * kv_heads;
   } else {
     return fail(LFM3A_EINVAL, "unknown cache mode");
   }
@@ -1174,6 +1183,394 @@ int lfm3a_pseq_blocks(const lfm3a_pseq* seq, int32_t* full, int32_t* slide, int 
     if (slide) slide[i] = seq->seq.slide[i];
   }
   return n;
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------- 8-bit block cache and eviction
+namespace {
+
+int check_view8(const lfm3a_kv8_view* kv) {
+  if (!kv) return fail(LFM3A_EINVAL, "null kv8 view");
+  const int rc = check_view(&kv->kv, true);
+  if (rc != LFM3A_OK) return rc;
+  if (!kv->tail || !aligned16(kv->tail)) return fail(LFM3A_EINVAL, "null or misaligned tail");
+  return LFM3A_OK;
+}
+
+// sealed: a multiple of the block, at most len, the rest within the tail.
+int check_sealed(int sealed, int len) {
+  if (sealed < 0 || sealed % kBlockTokens != 0) return fail(LFM3A_EINVAL, "sealed must be a multiple of 32 tokens");
+  if (len - sealed > kTailTokens) return fail(LFM3A_EINVAL, "more than 128 tokens past the sealed ones");
+  return LFM3A_OK;
+}
+
+// Calls f with the kernel arguments' (head_dim, format) as compile-time constants.
+template <typename F>
+int with_format(const lfm3a_kv_layout& L, F f) {
+  const bool e4m3 = L.mode == LFM3A_MODE_E4M3BLK;
+  if (L.head_dim == 64)
+    return e4m3 ? f(std::integral_constant<int, 64>{}, std::true_type{}) : f(std::integral_constant<int, 64>{}, std::false_type{});
+  return e4m3 ? f(std::integral_constant<int, 128>{}, std::true_type{}) : f(std::integral_constant<int, 128>{}, std::false_type{});
+}
+
+int kv8_rows_per_group(int rows) { return rows <= 8 ? 8 : rows <= 16 ? 16 : 32; }
+
+// Key splits of kv8_attend_kernel: whole waves of its resident blocks (two per SM at head_dim 64, one at 128), at least
+// a page for each of a block's warps.
+int kv8_splits_for(int kv_heads, int head_dim, int rows, int pages, int sm_count) {
+  const int groups = kv_heads * ((rows + kv8_rows_per_group(rows) - 1) / kv8_rows_per_group(rows));
+  const int nr = kv8_rows_per_group(rows);
+  const bool wide = head_dim == 64 && nr == 32;
+  const int target = (head_dim == 64 && !wide ? 2 : 1) * sm_count, warps = wide ? 12 : 8;
+  const int splits = std::max(1, target / groups);
+  return std::min(std::min(splits, std::max(1, (pages + warps - 1) / warps)), kKv8MaxSplits);
+}
+
+int kv8_pages(int ctx_len, int m, int window, int* begin) {
+  const int start = window > 0 ? std::max(0, ctx_len - window + 1) : 0;
+  *begin = start / kBlockTokens;
+  return (ctx_len + m - 1) / kBlockTokens - *begin + 1;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t lfm3a_kv8_tail_bytes(const lfm3a_kv_layout* layout) {
+  if (!layout || !is_block8(layout->mode) || layout->kv_heads <= 0 || layout->head_dim <= 0) return 0;
+  return (size_t)2 * layout->kv_heads * kTailTokens * layout->head_dim * sizeof(__half);
+}
+
+int lfm3a_kv8_append(const lfm3a_kv8_view* kv, const void* k, const void* v, int64_t token_stride, int pos0, int n,
+                     int sealed, int seal_to, const void* rope, const void* k_norm, void* stream) {
+  int rc = check_view8(kv);
+  if (rc != LFM3A_OK) return rc;
+  const lfm3a_kv_layout& L = kv->kv.layout;
+  const int D = L.head_dim, H = L.kv_heads;
+  if (n < 0 || pos0 < 0 || (n > 0 && (!k || !v))) return fail(LFM3A_EINVAL, "bad append arguments");
+  if (n > INT32_MAX - pos0 - kBlockTokens) return fail(LFM3A_EINVAL, "positions past 2^31");
+  if (token_stride == 0) token_stride = (int64_t)H * D;
+  if (token_stride < (int64_t)H * D) return fail(LFM3A_EINVAL, "token_stride smaller than kv_heads * head_dim");
+  const int len = pos0 + n;
+  if (pos0 < sealed) return fail(LFM3A_EINVAL, "the new tokens start below the sealed ones");
+  rc = check_sealed(sealed, pos0);
+  if (rc != LFM3A_OK) return rc;
+  if (seal_to < sealed || seal_to > len) return fail(LFM3A_EINVAL, "seal_to must lie between sealed and pos0 + n");
+  const int page0 = sealed / kBlockTokens, seal_end = seal_to / kBlockTokens;
+  const int page_end = (len + kBlockTokens - 1) / kBlockTokens;
+  rc = check_sealed(seal_end * kBlockTokens, len);
+  if (rc != LFM3A_OK) return rc;
+  Kv8AppendArgs a;
+  a.a.g = geom_of(&kv->kv);
+  a.a.k = static_cast<const __half*>(k);
+  a.a.v = static_cast<const __half*>(v);
+  a.a.rope = static_cast<const __half*>(rope);
+  a.a.knorm = static_cast<const __half*>(k_norm);
+  a.a.stride = token_stride;
+  a.a.pos0 = pos0;
+  a.a.n = n;
+  a.tail = static_cast<__half*>(kv->tail);
+  a.seal_page_end = seal_end;
+  const cudaStream_t st = as_stream(stream);
+  auto run = [&](int p0, int p1) -> int {
+    if (p1 <= p0) return LFM3A_OK;
+    a.page0 = p0;
+    rc = with_format(L, [&](auto d, auto f) {
+      launch_pdl(kv8_append_kernel<decltype(d)::value, decltype(f)::value>, dim3(p1 - p0, H), kSealThreads, 0, st, a);
+      return LFM3A_OK;
+    });
+    return check_launch("kv8_append_kernel");
+  };
+  // One launch, unless new tokens would go to tail slots that pages being sealed still read.
+  const int last = n > 0 ? page_end : seal_end;
+  if (pos0 == sealed || len - sealed <= kTailTokens) return run(page0, last);
+  rc = run(page0, seal_end);
+  return rc != LFM3A_OK ? rc : run(seal_end, last);
+}
+
+int lfm3a_kv8_read(const lfm3a_kv8_view* kv, int pos0, int n, int sealed, void* k, void* v, void* stream) {
+  int rc = check_view8(kv);
+  if (rc != LFM3A_OK) return rc;
+  if (n == 0) return LFM3A_OK;
+  if (!k || !v || n < 0 || pos0 < 0 || n > INT32_MAX - pos0) return fail(LFM3A_EINVAL, "bad read arguments");
+  if (!aligned16(k) || !aligned16(v)) return fail(LFM3A_EINVAL, "k and v must be 16-byte aligned");
+  rc = check_sealed(sealed, pos0 + n);
+  if (rc != LFM3A_OK) return rc;
+  const lfm3a_kv_layout& L = kv->kv.layout;
+  Kv8ReadArgs a{geom_of(&kv->kv), static_cast<__half*>(kv->tail), static_cast<__half*>(k), static_cast<__half*>(v),
+                pos0, n, sealed};
+  const dim3 grid((pos0 + n - 1) / kBlockTokens - pos0 / kBlockTokens + 1, L.kv_heads);
+  with_format(L, [&](auto d, auto f) {
+    launch_pdl(kv8_read_kernel<decltype(d)::value, decltype(f)::value>, grid, 256, 0, as_stream(stream), a);
+    return 0;
+  });
+  return check_launch("kv8_read_kernel");
+}
+
+int lfm3a_kv8_splits(const lfm3a_kv_layout* layout, int q_heads, int ctx_len, int m, int window, int sm_count) {
+  if (!layout || layout->kv_heads <= 0 || q_heads < layout->kv_heads || ctx_len < 0 || m < 1 || window < 0)
+    return fail(LFM3A_EINVAL, "bad kv8 split arguments");
+  int begin;
+  const int pages = kv8_pages(ctx_len, m, window, &begin);
+  return kv8_splits_for(layout->kv_heads, layout->head_dim, m * (q_heads / layout->kv_heads), pages,
+                        sm_count > 0 ? sm_count : current_sm_count());
+}
+
+int lfm3a_kv8_attention(const lfm3a_kv8_view* kv, const void* q, int64_t q_stride, int m, int q_heads, int ctx_len,
+                        int sealed, int window, const void* gate, void* out, float* lse, void* workspace,
+                        size_t workspace_bytes, int splits, void* stream) {
+  int rc = check_view8(kv);
+  if (rc != LFM3A_OK) return rc;
+  const lfm3a_kv_layout& L = kv->kv.layout;
+  const int D = L.head_dim, H = L.kv_heads;
+  if (!q || !out || m < 1 || ctx_len < 0 || window < 0 || ctx_len > INT32_MAX - 64 - m)
+    return fail(LFM3A_EINVAL, "bad attention arguments");
+  if (q_heads <= 0 || q_heads % H != 0) return fail(LFM3A_EINVAL, "q_heads must be a multiple of kv_heads");
+  const int group = q_heads / H;
+  if (m > 32 || (int64_t)m * group > LFM3A_KV8_MAX_ROWS)
+    return fail(LFM3A_ENOTSUP, "kv8 attention takes up to 32 tokens and 256 query rows per kv head");
+  if (q_stride == 0) q_stride = (int64_t)q_heads * D;
+  if (q_stride < (int64_t)q_heads * D || q_stride % 8 != 0)
+    return fail(LFM3A_EINVAL, "q_stride must be a multiple of 8 and at least q_heads * head_dim");
+  if (!aligned16(q) || !aligned16(out)) return fail(LFM3A_EINVAL, "q and out must be 16-byte aligned");
+  rc = check_sealed(sealed, ctx_len + m);
+  if (rc != LFM3A_OK) return rc;
+  Kv8AttnArgs a;
+  a.g = geom_of(&kv->kv);
+  a.tail = static_cast<__half*>(kv->tail);
+  a.q = static_cast<const __half*>(q);
+  a.gate = static_cast<const __half*>(gate);
+  a.out = static_cast<__half*>(out);
+  a.lse = lse;
+  a.q_stride = q_stride;
+  a.m = m;
+  a.group = group;
+  a.q_heads = q_heads;
+  a.ctx_len = ctx_len;
+  a.window = window;
+  a.sealed = sealed;
+  a.p_total = kv8_pages(ctx_len, m, window, &a.p_begin);
+  a.qk_scale = (1.f / sqrtf((float)D)) * kLog2e;
+  const int rows = m * group;
+  if (splits <= 0) splits = kv8_splits_for(H, D, rows, a.p_total, current_sm_count());
+  a.splits = std::min(std::min(splits, a.p_total), kKv8MaxSplits);
+  a.part = nullptr;
+  if (a.splits > 1) {
+    if (!workspace || !aligned16(workspace)) return fail(LFM3A_EINVAL, "kv8 attention needs a 16-byte aligned workspace");
+    if (workspace_bytes < lfm3a_verify_workspace_bytes(m, q_heads, D, a.splits))
+      return fail(LFM3A_EWORKSPACE, "kv8 attention workspace too small");
+    a.part = static_cast<float*>(workspace);
+  }
+  const cudaStream_t st = as_stream(stream);
+  static std::atomic<bool> done[12][64];
+  const int nr = kv8_rows_per_group(rows);
+  const dim3 grid(a.splits, H, (rows + nr - 1) / nr);
+  rc = with_format(L, [&](auto d, auto f) {
+    constexpr int DD = decltype(d)::value;
+    constexpr bool E = decltype(f)::value;
+    constexpr int slot = (DD == 64 ? 0 : 6) + (E ? 3 : 0);
+    auto run = [&](auto kernel, int smem, int threads, int i) {
+      const int r = ensure_smem(kernel, smem, done[slot + i]);
+      if (r == LFM3A_OK) launch_pdl(kernel, grid, threads, smem, st, a);
+      return r;
+    };
+    if (nr == 8) return run(kv8_attend_kernel<DD, 1, E>, Kv8Attn<DD, 1>::kSmem, Kv8Attn<DD, 1>::kThreads, 0);
+    if (nr == 16) return run(kv8_attend_kernel<DD, 2, E>, Kv8Attn<DD, 2>::kSmem, Kv8Attn<DD, 2>::kThreads, 1);
+    return run(kv8_attend_kernel<DD, 4, E>, Kv8Attn<DD, 4>::kSmem, Kv8Attn<DD, 4>::kThreads, 2);
+  });
+  if (rc != LFM3A_OK) return rc;
+  rc = check_launch("kv8_attend_kernel");
+  if (rc != LFM3A_OK || a.splits == 1) return rc;
+  if (D == 64) launch_pdl(kv8_combine_kernel<64>, m * q_heads, kKv8CombineThreads, 0, st, a.part, a.splits, a.gate, a.out, lse);
+  else launch_pdl(kv8_combine_kernel<128>, m * q_heads, kKv8CombineThreads, 0, st, a.part, a.splits, a.gate, a.out, lse);
+  return check_launch("kv8_combine_kernel");
+}
+
+// Prefill workspace: the staged sections, their block table and scales, the key splits' partials.
+static size_t kv8_stage_bytes(int kv_heads, int head_dim, int pages) {
+  return (size_t)pages * kv_heads * (head_dim == 64 ? kStagedHeadBytes<64> : kStagedHeadBytes<128>);
+}
+static size_t kv8_table_bytes(int pages) { return ((size_t)pages * sizeof(int32_t) + 255) / 256 * 256; }
+static size_t kv8_scale_bytes(int kv_heads, int pages) { return (size_t)pages * kv_heads * sizeof(float4); }
+
+size_t lfm3a_kv8_prefill_workspace_bytes(const lfm3a_kv_layout* layout, int tokens, int q_heads, int max_len) {
+  if (!layout || !is_block8(layout->mode) || tokens <= 0 || max_len <= 0 || q_heads < layout->kv_heads) return 0;
+  const int pages = (max_len + kBlockTokens - 1) / kBlockTokens + 2, D = layout->head_dim;
+  const size_t staged = kv8_stage_bytes(layout->kv_heads, D, pages) + kv8_table_bytes(pages) +
+                        kv8_scale_bytes(layout->kv_heads, pages) + lfm3a_prefill_workspace_bytes(tokens, q_heads, D);
+  // A call that goes 32 tokens at a time needs one call's split partials.
+  const int rows = 32 * (q_heads / layout->kv_heads);
+  const int splits = kv8_splits_for(layout->kv_heads, D, rows, pages, current_sm_count());
+  return std::max(staged, lfm3a_verify_workspace_bytes(32, q_heads, D, splits) * 2);
+}
+
+int lfm3a_kv8_prefill(const lfm3a_kv8_view* kv, const void* q, int64_t q_stride, int tokens, int q_heads, int context,
+                      int sealed, int window, void* out, void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = check_view8(kv);
+  if (rc != LFM3A_OK) return rc;
+  const lfm3a_kv_layout& L = kv->kv.layout;
+  const int D = L.head_dim, H = L.kv_heads;
+  if (!q || !out || tokens < 0 || context < 0 || window < 0 || tokens > INT32_MAX - 128 - context)
+    return fail(LFM3A_EINVAL, "bad prefill arguments");
+  if (q_heads <= 0 || q_heads % H != 0) return fail(LFM3A_EINVAL, "q_heads must be a multiple of kv_heads");
+  if (q_stride == 0) q_stride = (int64_t)q_heads * D;
+  if (q_stride < (int64_t)q_heads * D || q_stride % 8 != 0)
+    return fail(LFM3A_EINVAL, "q_stride must be a multiple of 8 and at least q_heads * head_dim");
+  if (!aligned16(q) || !aligned16(out)) return fail(LFM3A_EINVAL, "q and out must be 16-byte aligned");
+  const int len = context + tokens, group = q_heads / H;
+  rc = check_sealed(sealed, len);
+  if (rc != LFM3A_OK || tokens == 0) return rc;
+  if (!workspace || !aligned16(workspace)) return fail(LFM3A_EINVAL, "kv8 prefill needs a 16-byte aligned workspace");
+  if (tokens <= 32 || group != 4) {
+    const int step = std::min(32, std::max(1, LFM3A_KV8_MAX_ROWS / group));
+    // Every slice's workspace is checked before the first launch.
+    for (int pass = 0; pass < 2; ++pass)
+      for (int t = 0; t < tokens; t += step) {
+        const int m = std::min(step, tokens - t);
+        if (pass == 0) {
+          const int splits = lfm3a_kv8_splits(&L, q_heads, context + t, m, window, 0);
+          if (splits > 1 && workspace_bytes < lfm3a_verify_workspace_bytes(m, q_heads, D, splits))
+            return fail(LFM3A_EWORKSPACE, "kv8 prefill workspace too small");
+          continue;
+        }
+        rc = lfm3a_kv8_attention(kv, static_cast<const __half*>(q) + t * q_stride, q_stride, m, q_heads, context + t,
+                                 sealed, window, nullptr, static_cast<__half*>(out) + (int64_t)t * q_heads * D, nullptr,
+                                 workspace, workspace_bytes, 0, stream);
+        if (rc != LFM3A_OK) return rc;
+      }
+    return LFM3A_OK;
+  }
+  // Stage the pages any token sees as MODE_F16 sections (whole 64-key tiles), then the exact prefill kernel.
+  const int start = window > 0 ? std::max(0, context - window + 1) : 0;
+  const int page0 = start / kQuantBlock * (kQuantBlock / kBlockTokens), pages = (len + kBlockTokens - 1) / kBlockTokens;
+  const int staged = pages - page0;
+  const size_t at_table = kv8_stage_bytes(H, D, staged), at_scales = at_table + kv8_table_bytes(pages);
+  const size_t at_part = at_scales + kv8_scale_bytes(H, staged);
+  if (workspace_bytes < at_part) return fail(LFM3A_EWORKSPACE, "kv8 prefill workspace too small");
+  Kv8ExpandArgs e;
+  e.g = geom_of(&kv->kv);
+  e.tail = static_cast<__half*>(kv->tail);
+  e.dst = static_cast<char*>(workspace);
+  e.table = reinterpret_cast<int32_t*>(static_cast<char*>(workspace) + at_table);
+  e.scales = reinterpret_cast<float4*>(static_cast<char*>(workspace) + at_scales);
+  e.page0 = page0;
+  e.sealed = sealed;
+  e.len = len;
+  const cudaStream_t st = as_stream(stream);
+  with_format(L, [&](auto d, auto f) {
+    launch_pdl(kv8_expand_kernel<decltype(d)::value, decltype(f)::value>, dim3(staged, H), 256, 0, st, e);
+    return 0;
+  });
+  rc = check_launch("kv8_expand_kernel");
+  if (rc != LFM3A_OK) return rc;
+  KvGeom g;
+  g.pool = e.dst;
+  g.table = e.table;
+  g.pool_blocks = staged;
+  g.head_bytes = D == 64 ? kStagedHeadBytes<64> : kStagedHeadBytes<128>;
+  g.block_bytes = g.head_bytes * H;
+  g.kv_heads = H;
+  int splits = prefill_splits_for(tokens, H, context, window, current_sm_count(), 2);
+  const size_t need = (size_t)tokens * q_heads * splits * (D + 2) * sizeof(float);
+  if (splits > 1 && workspace_bytes < at_part + need) splits = 1;
+  float* part = splits > 1 ? reinterpret_cast<float*>(static_cast<char*>(workspace) + at_part) : nullptr;
+  rc = launch_prefill(g, static_cast<const __half*>(q), q_stride, nullptr, nullptr, nullptr, 0, tokens, q_heads, context,
+                      window, true, static_cast<__half*>(out), splits, part, st, D, e.scales, page0);
+  if (rc != LFM3A_OK || splits == 1) return rc;
+  return launch_combine(part, tokens * q_heads, splits, D, D + 2, (int64_t)splits * (D + 2), nullptr,
+                        static_cast<__half*>(out), nullptr, st);
+}
+
+int lfm3a_kv8_weights(const lfm3a_kv8_view* kv, const void* q, int64_t q_stride, int m, int q_heads, int ctx_len,
+                      int sealed, int window, const float* lse, const float* prev, int64_t prev_stride, float decay,
+                      float* out, int64_t out_stride, void* stream) {
+  int rc = check_view8(kv);
+  if (rc != LFM3A_OK) return rc;
+  const lfm3a_kv_layout& L = kv->kv.layout;
+  const int D = L.head_dim, H = L.kv_heads;
+  if (!q || !lse || !out || m < 1 || ctx_len < 0 || window < 0 || ctx_len > INT32_MAX - 64 - m)
+    return fail(LFM3A_EINVAL, "bad weight arguments");
+  if (q_heads <= 0 || q_heads % H != 0) return fail(LFM3A_EINVAL, "q_heads must be a multiple of kv_heads");
+  const int group = q_heads / H;
+  if (m > 32 || (int64_t)m * group > LFM3A_KV8_MAX_ROWS)
+    return fail(LFM3A_ENOTSUP, "kv8 weights take up to 32 tokens and 256 query rows per kv head");
+  if (q_stride == 0) q_stride = (int64_t)q_heads * D;
+  if (q_stride < (int64_t)q_heads * D || q_stride % 8 != 0)
+    return fail(LFM3A_EINVAL, "q_stride must be a multiple of 8 and at least q_heads * head_dim");
+  if (!aligned16(q)) return fail(LFM3A_EINVAL, "q must be 16-byte aligned");
+  const int len = ctx_len + m;
+  if (out_stride < len || (prev && prev_stride < len)) return fail(LFM3A_EINVAL, "a row of weights is shorter than the sequence");
+  rc = check_sealed(sealed, len);
+  if (rc != LFM3A_OK) return rc;
+  Kv8WeightArgs a;
+  a.g = geom_of(&kv->kv);
+  a.tail = static_cast<__half*>(kv->tail);
+  a.q = static_cast<const __half*>(q);
+  a.lse = lse;
+  a.prev = prev;
+  a.out = out;
+  a.q_stride = q_stride;
+  a.prev_stride = prev_stride;
+  a.out_stride = out_stride;
+  a.m = m;
+  a.group = group;
+  a.q_heads = q_heads;
+  a.ctx_len = ctx_len;
+  a.window = window;
+  a.sealed = sealed;
+  a.pages = (len + kBlockTokens - 1) / kBlockTokens;
+  a.decay = decay;
+  a.qk_scale = (1.f / sqrtf((float)D)) * kLog2e;
+  const int target = (D == 64 ? 2 : 1) * current_sm_count();
+  a.splits = std::max(1, std::min(target / H, (a.pages + 7) / 8));
+  const int ntiles = (m * group + 7) / 8;
+  const cudaStream_t st = as_stream(stream);
+  static std::atomic<bool> done[4][64];
+  rc = with_format(L, [&](auto d, auto f) {
+    constexpr int DD = decltype(d)::value;
+    constexpr bool E = decltype(f)::value;
+    using W = Kv8Weights<DD>;
+    const int r = ensure_smem(kv8_weights_kernel<DD, E>, W::smem(W::kMaxRows / 8), done[(DD == 64 ? 0 : 2) + (E ? 1 : 0)]);
+    if (r == LFM3A_OK)
+      launch_pdl(kv8_weights_kernel<DD, E>, dim3(a.splits, H), W::kThreads, W::smem(ntiles), st, a);
+    return r;
+  });
+  if (rc != LFM3A_OK) return rc;
+  return check_launch("kv8_weights_kernel");
+}
+
+int lfm3a_evict_select(const float* weights, int64_t stride, int kv_heads, int len, int sink, int recent, int budget,
+                       int32_t* keep, float* weights_out, int64_t out_stride, void* stream) {
+  if (!weights || !keep || kv_heads < 1 || kv_heads > 65535 || len < 1) return fail(LFM3A_EINVAL, "bad eviction arguments");
+  if (stride < len || (weights_out && out_stride < budget)) return fail(LFM3A_EINVAL, "a row of weights is too short");
+  if (sink < 0 || recent < 0 || budget < 1 || budget > len || (int64_t)sink + recent > budget)
+    return fail(LFM3A_EINVAL, "need sink + recent <= budget <= len");
+  EvictArgs a{weights, keep, weights_out, stride, out_stride, len, sink, recent, budget};
+  launch_pdl(evict_select_kernel, dim3(kEvictCluster, kv_heads), kEvictThreads, 0, as_stream(stream), a);
+  return check_launch("evict_select_kernel");
+}
+
+int lfm3a_kv8_compact(const lfm3a_kv8_view* src, int len, int sealed, const int32_t* keep, int budget,
+                      const lfm3a_kv8_view* dst, void* stream) {
+  int rc = check_view8(src);
+  if (rc == LFM3A_OK) rc = check_view8(dst);
+  if (rc != LFM3A_OK) return rc;
+  const lfm3a_kv_layout &L = src->kv.layout, &M = dst->kv.layout;
+  if (L.mode != M.mode || L.kv_heads != M.kv_heads || L.head_dim != M.head_dim)
+    return fail(LFM3A_EINVAL, "compaction needs two caches of one layout");
+  if (!keep || len < 1 || budget < 1 || budget > len) return fail(LFM3A_EINVAL, "bad compaction arguments");
+  if (src->tail == dst->tail) return fail(LFM3A_EINVAL, "compaction into the same cache");
+  rc = check_sealed(sealed, len);
+  if (rc != LFM3A_OK) return rc;
+  Kv8CompactArgs a{geom_of(&src->kv), geom_of(&dst->kv), static_cast<__half*>(src->tail), static_cast<__half*>(dst->tail),
+                   keep, len, sealed, budget};
+  const dim3 grid((budget + kBlockTokens - 1) / kBlockTokens, L.kv_heads);
+  with_format(L, [&](auto d, auto f) {
+    launch_pdl(kv8_compact_kernel<decltype(d)::value, decltype(f)::value>, grid, kSealThreads, 0, as_stream(stream), a);
+    return 0;
+  });
+  return check_launch("kv8_compact_kernel");
 }
 
 }  // extern "C"

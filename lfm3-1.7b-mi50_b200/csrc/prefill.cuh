@@ -73,6 +73,8 @@ struct PrefillArgs {
   int64_t q_stride, gate_stride;
   int T, q_heads, context, window, qtiles, splits;
   float qk_scale;         // (1 / sqrt(64)) * log2(e)
+  const float4* scales = nullptr;   // SCALED: (K factor, log2 of the V factor, its reciprocal, -) of page p, head h at
+  int scale_page0 = 0;              // [(p - scale_page0) * kv_heads + h]
 };
 
 // Query row (tok, qh) into its core tiles: row r, dims 8c .. 8c + 7 at ((r / 8) * 8 + c) * 128 + (r % 8) * 16.
@@ -270,7 +272,10 @@ struct PfLayout {
 // carries none of that code, so the tile loops keep their register allocation.
 // GLUE: the launch fuses the q-norm / RoPE of the query rows or the output gate (lfm3a_prefill_attention_fused);
 // the plain instantiation reads Q as it is and stores the output ungated.
-template <int D, bool I8, bool SPLIT, bool GLUE>
+// SCALED (exact only): the pool's K and V are 8-bit codes as fp16 with one factor per page and head (kv8.cuh): the K
+// factor multiplies the page's scores, the V factor goes into their exponents (P' = 2^(s + log2 f - m)), whose sum is
+// taken over P' / f, after its rounding to fp16, so that numerator and denominator carry the same roundings.
+template <int D, bool I8, bool SPLIT, bool GLUE, bool SCALED = false>
 __global__ __launch_bounds__(PfLayout<D, I8>::kThreads, PfLayout<D, I8>::kBlocksPerSm) void prefill_kernel(PrefillArgs a) {
   using L = PfLayout<D, I8>;
   constexpr int NS = L::kStages;
@@ -382,8 +387,27 @@ __global__ __launch_bounds__(PfLayout<D, I8>::kThreads, PfLayout<D, I8>::kBlocks
     float m_run = -INFINITY, l_run = 0.f;
     // Every wait result is made warp-uniform: the tcgen05.ld/st that follow are warp-collective.
     bool ok = true;
+    // The factors of the tile's two pages, loaded a tile ahead (a page past the keys: the first page's).
+    float4 sc_next[2];
+    auto load_scales = [&](int jt) {
+      const int lp0 = (kt_begin + jt * kQuantBlock) / kBlockTokens;
+      const int lp1 = (lp0 + 1) * kBlockTokens < kend ? lp0 + 1 : lp0;
+      sc_next[0] = a.scales[(int64_t)(lp0 - a.scale_page0) * a.g.kv_heads + h];
+      sc_next[1] = a.scales[(int64_t)(lp1 - a.scale_page0) * a.g.kv_heads + h];
+    };
+    if constexpr (SCALED) load_scales(0);
     for (int jt = 0; jt < ntiles && ok; ++jt) {
       const int b = jt & 1, k0 = kt_begin + jt * kQuantBlock;
+      float kf[2], vl[2], vr[2];
+      if constexpr (SCALED) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          kf[i] = sc_next[i].x * a.qk_scale;
+          vl[i] = sc_next[i].y;
+          vr[i] = sc_next[i].z;
+        }
+        if (jt + 1 < ntiles) load_scales(jt + 1);
+      }
       if (!__all_sync(0xffffffffu, mbar_wait(&s_full[b], (uint32_t)(jt >> 1) & 1u))) {
         raise_error(kErrWaitMma);
         ok = false;
@@ -409,7 +433,9 @@ __global__ __launch_bounds__(PfLayout<D, I8>::kThreads, PfLayout<D, I8>::kBlocks
         for (int k = 0; k < 64; ++k) x[k] = (k >= lo && k <= hi) ? x[k] : -INFINITY;
       }
       // fl(x * scale) is monotone in x, so the scaled maximum is the maximum of the scaled scores.
-      const float mx = max64(x) * a.qk_scale;
+      float mx;
+      if constexpr (SCALED) mx = fmaxf(fmaf(max32(x), kf[0], vl[0]), fmaf(max32(x + 32), kf[1], vl[1]));
+      else mx = max64(x) * a.qk_scale;
       const bool grow_max = mx > m_run + kLazy;
       // O lives in TMEM: rescaling it needs the previous PV finished; rare after the first tiles.
       if (__any_sync(0xffffffffu, grow_max)) {
@@ -439,17 +465,31 @@ __global__ __launch_bounds__(PfLayout<D, I8>::kThreads, PfLayout<D, I8>::kBlocks
       // p = 2^(x * scale - m) in one FFMA + EX2 (ex2 of -inf is 0 for masked keys); l in four partial sums.
       // Pairs of keys in packed fp32 (ls01 and ls23 sum keys 4i, 4i + 1 and 4i + 2, 4i + 3).
       const float neg = m_run == -INFINITY ? 0.f : -m_run;
-      const float2 sc2 = make_float2(a.qk_scale, a.qk_scale), neg2 = make_float2(neg, neg);
-      float2 ls01 = make_float2(0.f, 0.f), ls23 = make_float2(0.f, 0.f);
+      uint32_t pw[SCALED ? 32 : 1];   // SCALED: P as fp16 pairs
+      if constexpr (SCALED) {
+        float2 ls[2][2] = {};
 #pragma unroll
-      for (int k = 0; k < 64; k += 2) {
-        const float2 g = ffma2(make_float2(x[k], x[k + 1]), sc2, neg2);
-        x[k] = fast_exp2(g.x);
-        x[k + 1] = fast_exp2(g.y);
-        if (k & 2) ls23 = fadd2(ls23, make_float2(x[k], x[k + 1]));
-        else ls01 = fadd2(ls01, make_float2(x[k], x[k + 1]));
+        for (int k = 0; k < 64; k += 2) {
+          const int i = k >> 5;
+          const float2 g = ffma2(make_float2(x[k], x[k + 1]), make_float2(kf[i], kf[i]), make_float2(vl[i] + neg, vl[i] + neg));
+          pw[k / 2] = pack_half2(fast_exp2(g.x), fast_exp2(g.y));
+          ls[i][(k >> 1) & 1] = fadd2(ls[i][(k >> 1) & 1], unpack_half2(pw[k / 2]));
+        }
+        const float2 l0 = fadd2(ls[0][0], ls[0][1]), l1 = fadd2(ls[1][0], ls[1][1]);
+        l_run = fmaf(l0.x + l0.y, vr[0], fmaf(l1.x + l1.y, vr[1], l_run));
+      } else {
+        const float2 sc2 = make_float2(a.qk_scale, a.qk_scale), neg2 = make_float2(neg, neg);
+        float2 ls01 = make_float2(0.f, 0.f), ls23 = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < 64; k += 2) {
+          const float2 g = ffma2(make_float2(x[k], x[k + 1]), sc2, neg2);
+          x[k] = fast_exp2(g.x);
+          x[k + 1] = fast_exp2(g.y);
+          if (k & 2) ls23 = fadd2(ls23, make_float2(x[k], x[k + 1]));
+          else ls01 = fadd2(ls01, make_float2(x[k], x[k + 1]));
+        }
+        l_run += (ls01.x + ls01.y) + (ls23.x + ls23.y);
       }
-      l_run += (ls01.x + ls01.y) + (ls23.x + ls23.y);
       // P[b] was last read by PV(jt - 2), issued before QK(jt): the commit that signalled S(jt) covers it.
       // With one P buffer, PV(jt - 1) must have read it: wait for its commit (already done when O was rescaled).
       if (L::kPBufs == 1 && jt >= 1 &&
@@ -462,10 +502,14 @@ __global__ __launch_bounds__(PfLayout<D, I8>::kThreads, PfLayout<D, I8>::kBlocks
 #pragma unroll
       for (int c = 0; c < 8; ++c) {
         uint4 v;
-        v.x = pack_half2(x[8 * c], x[8 * c + 1]);
-        v.y = pack_half2(x[8 * c + 2], x[8 * c + 3]);
-        v.z = pack_half2(x[8 * c + 4], x[8 * c + 5]);
-        v.w = pack_half2(x[8 * c + 6], x[8 * c + 7]);
+        if constexpr (SCALED) {
+          v = make_uint4(pw[4 * c], pw[4 * c + 1], pw[4 * c + 2], pw[4 * c + 3]);
+        } else {
+          v.x = pack_half2(x[8 * c], x[8 * c + 1]);
+          v.y = pack_half2(x[8 * c + 2], x[8 * c + 3]);
+          v.z = pack_half2(x[8 * c + 4], x[8 * c + 5]);
+          v.w = pack_half2(x[8 * c + 6], x[8 * c + 7]);
+        }
         *reinterpret_cast<uint4*>(pb + ((r >> 3) * 8 + c) * 128 + (r & 7) * 16) = v;
       }
       fence_proxy_async_smem();
@@ -917,7 +961,7 @@ __global__ __launch_bounds__(PfLayout<D, I8>::kThreads, PfLayout<D, I8>::kBlocks
 }
 
 inline int launch_prefill_kernel(const PrefillArgs& a, bool i8, int head_dim, cudaStream_t st) {
-  static std::atomic<bool> done[16][64];   // per device: set once the attributes are (see ensure_smem)
+  static std::atomic<bool> done[20][64];   // per device: set once the attributes are (see ensure_smem)
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return LFM3A_ECUDA;
   const dim3 grid(a.qtiles, a.g.kv_heads, a.splits);
@@ -933,7 +977,14 @@ inline int launch_prefill_kernel(const PrefillArgs& a, bool i8, int head_dim, cu
     return true;
   };
   bool ok;
-  if (head_dim == 128) {   // the reference model's geometry
+  if (a.scales) {   // the 8-bit block cache's staged codes (exact, no glue)
+    using L1 = PfLayout<128, false>;
+    using L0 = PfLayout<64, false>;
+    if (head_dim == 128) ok = split ? run(prefill_kernel<128, false, true, false, true>, L1::kRequest, L1::kThreads, 19)
+                                    : run(prefill_kernel<128, false, false, false, true>, L1::kRequest, L1::kThreads, 18);
+    else ok = split ? run(prefill_kernel<64, false, true, false, true>, L0::kRequest, L0::kThreads, 17)
+                    : run(prefill_kernel<64, false, false, false, true>, L0::kRequest, L0::kThreads, 16);
+  } else if (head_dim == 128) {   // the reference model's geometry
     using LI = PfLayout<128, true>;
     using LE = PfLayout<128, false>;
     if (i8) {
@@ -997,8 +1048,11 @@ inline int prefill_splits_for(int tokens, int kv_heads, int context, int window,
 // if any, is left to prefill_gate_kernel after it).
 inline int launch_prefill(const KvGeom& g, const __half* q, int64_t q_stride, const __half* q_norm, const __half* rope,
                           const __half* gate, int64_t gate_stride, int tokens, int q_heads, int context, int window,
-                          bool exact, __half* out, int splits, float* part, cudaStream_t st, int head_dim = 64) {
+                          bool exact, __half* out, int splits, float* part, cudaStream_t st, int head_dim = 64,
+                          const float4* scales = nullptr, int scale_page0 = 0) {
   PrefillArgs a;
+  a.scales = scales;
+  a.scale_page0 = scale_page0;
   a.g = g;
   a.q = q;
   a.q_stride = q_stride;

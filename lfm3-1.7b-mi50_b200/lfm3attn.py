@@ -24,6 +24,8 @@ CUBIN_PATH = _HERE / "cubin" / "lfm3attn_sm100a.cubin"
 
 MODE_F16 = 0
 MODE_I8REC = 1
+MODE_I8BLK = 2
+MODE_E4M3BLK = 3
 BLOCK_TOKENS = 32
 QUANT_BLOCK = 64
 
@@ -56,8 +58,16 @@ class KvView(ctypes.Structure):
     ]
 
 
+class Kv8View(ctypes.Structure):
+    _fields_ = [
+        ("kv", KvView),
+        ("tail", ctypes.c_void_p),
+    ]
+
+
 _P = ctypes.c_void_p
 _I = ctypes.c_int
+_F = ctypes.c_float
 _I64 = ctypes.c_int64
 _SZ = ctypes.c_size_t
 
@@ -106,6 +116,16 @@ SIGNATURES = {
     "lfm3a_g128_gemm": (_I, [_P, _P, _P, _P, _I, _I, _I, _P, _I64, _P, _I64, _P]),
     "lfm3a_g128_workspace_bytes": (_I64, [_I, _I]),
     "lfm3a_g128_linear": (_I, [_P, _I64, _I, _I, _P, _P, _I, _I, _P, _I64, _P, _I64, _P, _SZ, _P]),
+    "lfm3a_kv8_tail_bytes": (_SZ, [ctypes.POINTER(KvLayout)]),
+    "lfm3a_kv8_append": (_I, [ctypes.POINTER(Kv8View), _P, _P, _I64, _I, _I, _I, _I, _P, _P, _P]),
+    "lfm3a_kv8_read": (_I, [ctypes.POINTER(Kv8View), _I, _I, _I, _P, _P, _P]),
+    "lfm3a_kv8_splits": (_I, [ctypes.POINTER(KvLayout), _I, _I, _I, _I, _I]),
+    "lfm3a_kv8_attention": (_I, [ctypes.POINTER(Kv8View), _P, _I64, _I, _I, _I, _I, _I, _P, _P, _P, _P, _SZ, _I, _P]),
+    "lfm3a_kv8_prefill_workspace_bytes": (_SZ, [ctypes.POINTER(KvLayout), _I, _I, _I]),
+    "lfm3a_kv8_prefill": (_I, [ctypes.POINTER(Kv8View), _P, _I64, _I, _I, _I, _I, _I, _P, _P, _SZ, _P]),
+    "lfm3a_kv8_weights": (_I, [ctypes.POINTER(Kv8View), _P, _I64, _I, _I, _I, _I, _I, _P, _P, _I64, _F, _P, _I64, _P]),
+    "lfm3a_evict_select": (_I, [_P, _I64, _I, _I, _I, _I, _I, _P, _P, _I64, _P]),
+    "lfm3a_kv8_compact": (_I, [ctypes.POINTER(Kv8View), _I, _I, _P, _I, ctypes.POINTER(Kv8View), _P]),
     "lfm3a_gather_region_bytes": (_SZ, [_I, _I, _I]),
     "lfm3a_gather_region_alloc": (_I, [_I, _I, _I, ctypes.POINTER(_P)]),
     "lfm3a_gather_region_free": (_I, [_P]),
@@ -447,6 +467,182 @@ class LayerCache:
         pool = self.pool.cpu().numpy()
         table = self.table.cpu().numpy()
         return decode_pool(pool, table, self.layout, length)
+
+
+class LayerCache8:
+    """One layer's 8-bit cache: a paged pool of MODE_I8BLK or MODE_E4M3BLK blocks (32 tokens, one scale per block and
+    kv head), its block table and the fp16 tail of the tokens that are not sealed yet (include/lfm3attn.h).
+
+    `length` tokens are cached, `sealed` of them in 8 bits. append seals every complete block of committed tokens;
+    tokens appended as drafts stay in the tail until a later append finds them committed (below its position)."""
+
+    def __init__(self, mode: int, kv_heads: int, head_dim: int, capacity_tokens: int, device="cuda", block_table=None,
+                 pool_blocks: int | None = None, pool=None):
+        """pool: another LayerCache8 of the same layout whose pool this one shares through its own block table."""
+        import torch
+
+        if mode not in (MODE_I8BLK, MODE_E4M3BLK):
+            raise LFM3AError(ENOTSUP, "LayerCache8 holds MODE_I8BLK or MODE_E4M3BLK")
+        self.layout = layout(mode, kv_heads, head_dim)
+        self.mode, self.kv_heads, self.head_dim = mode, kv_heads, head_dim
+        self.capacity = capacity_tokens
+        logical = (capacity_tokens + BLOCK_TOKENS - 1) // BLOCK_TOKENS
+        if pool is not None:
+            if pool.layout.block_bytes != self.layout.block_bytes or pool.mode != mode:
+                raise LFM3AError(EINVAL, "a shared pool needs the same layout")
+            self.pool_blocks, self.pool = pool.pool_blocks, pool.pool
+        else:
+            self.pool_blocks = pool_blocks if pool_blocks is not None else max(1, logical)
+            self.pool = torch.zeros(self.pool_blocks * self.layout.block_bytes, dtype=torch.uint8, device=device)
+        if block_table is None:
+            block_table = torch.arange(max(1, logical), dtype=torch.int32, device=device)
+        self.table = block_table
+        self.tail = torch.zeros(lib().lfm3a_kv8_tail_bytes(ctypes.byref(self.layout)), dtype=torch.uint8, device=device)
+        self.length = self.sealed = 0
+        self.view = Kv8View(KvView(self.pool.data_ptr(), self.table.data_ptr(), self.pool_blocks, self.layout),
+                            self.tail.data_ptr())
+        self._view = ctypes.byref(self.view)
+
+    def workspace(self, tokens: int, q_heads: int):
+        """A device workspace for verify (up to 32 tokens) and prefill calls of this many tokens at any length."""
+        import torch
+
+        need = lib().lfm3a_kv8_prefill_workspace_bytes(ctypes.byref(self.layout), tokens, q_heads, self.capacity)
+        if tokens <= 32:   # no staging
+            need = lib().lfm3a_verify_workspace_bytes(tokens, q_heads, self.head_dim, self.splits(q_heads, 1 << 30, tokens))
+        return torch.empty(need, dtype=torch.uint8, device=self.pool.device)
+
+    def splits(self, q_heads: int, ctx_len: int, m: int, window: int = 0) -> int:
+        rc = lib().lfm3a_kv8_splits(ctypes.byref(self.layout), q_heads, ctx_len, m, window, 0)
+        if rc < 0:
+            _check(rc)
+        return rc
+
+    def append(self, k, v, pos0: int | None = None, rope=None, k_norm=None, token_stride: int = 0, draft: bool = False,
+               stream=None) -> None:
+        """Stores k, v ([n][kv_heads][head_dim] fp16 device tensors) at positions pos0.. (default: the end). draft: the
+        new tokens may be rolled back, so only tokens below pos0 are sealed."""
+        pos0 = self.length if pos0 is None else pos0
+        n = k.shape[0]
+        if pos0 + n > self.capacity:
+            raise LFM3AError(EINVAL, "append past the cache capacity")
+        if pos0 > self.length:
+            raise LFM3AError(EINVAL, "append would leave a gap")
+        seal_to = pos0 if draft else pos0 + n
+        _check(lib().lfm3a_kv8_append(self._view, _ptr(k), _ptr(v), token_stride, pos0, n, self.sealed, seal_to,
+                                      _ptr(rope), _ptr(k_norm), _stream(stream)))
+        self.sealed = seal_to // BLOCK_TOKENS * BLOCK_TOKENS
+        self.length = pos0 + n
+
+    def truncate(self, new_len: int) -> None:
+        """Rollback after rejected drafts: the length drops; no device work."""
+        if not self.sealed <= new_len <= self.length:
+            raise LFM3AError(EINVAL, "truncate below the sealed tokens, or past the end")
+        self.length = new_len
+
+    def read(self, pos0: int, n: int, stream=None):
+        """(K, V) fp16 [n][kv_heads][head_dim]: the values the cached tokens pos0.. stand for."""
+        import torch
+
+        if pos0 < 0 or n < 0 or pos0 + n > self.length:
+            raise LFM3AError(EINVAL, "read past the cached tokens")
+        k, v = (torch.empty((n, self.kv_heads, self.head_dim), dtype=torch.float16, device=self.pool.device)
+                for _ in range(2))
+        _check(lib().lfm3a_kv8_read(self._view, pos0, n, self.sealed, _ptr(k), _ptr(v), _stream(stream)))
+        return k, v
+
+    def _check_q(self, q, ctx_len: int) -> tuple[int, int, int]:
+        m, qh, d = q.shape
+        if d != self.head_dim or q.stride(2) != 1 or (qh > 1 and q.stride(1) != d):
+            raise LFM3AError(EINVAL, "q must be [tokens][q_heads][head_dim] with contiguous rows")
+        if ctx_len < 0 or ctx_len + m > self.length:
+            raise LFM3AError(EINVAL, "the queries' tokens must be appended first")
+        return m, qh, q.stride(0) if m > 1 else qh * d
+
+    def verify(self, q, ctx_len: int, window: int = 0, gate=None, out=None, lse=None, workspace=None, splits: int = 0,
+               stream=None):
+        """Attention of q ([m][q_heads][head_dim] fp16, row-strided) at ctx_len.., m <= 32; the tokens' K/V appended.
+        lse: fp32 [m][q_heads] to fill with each row's log-sum-exp. Returns fp16 [m][q_heads][head_dim]."""
+        import torch
+
+        m, qh, stride = self._check_q(q, ctx_len)
+        if out is None:
+            out = torch.empty((m, qh, self.head_dim), dtype=torch.float16, device=q.device)
+        if workspace is None:
+            s = splits if splits > 0 else self.splits(qh, ctx_len, m, window)
+            workspace = torch.empty(lib().lfm3a_verify_workspace_bytes(m, qh, self.head_dim, s), dtype=torch.uint8,
+                                    device=q.device)
+        _check(lib().lfm3a_kv8_attention(self._view, _ptr(q), stride, m, qh, ctx_len, self.sealed_below(ctx_len + m),
+                                         window, _ptr(gate), _ptr(out), _ptr(lse), _ptr(workspace), workspace.numel(),
+                                         splits, _stream(stream)))
+        return out
+
+    def sealed_below(self, length: int) -> int:
+        """Sealed tokens as a call over the first `length` tokens takes them."""
+        return min(self.sealed, (length + BLOCK_TOKENS - 1) // BLOCK_TOKENS * BLOCK_TOKENS)
+
+    def prefill(self, q, context: int, window: int = 0, out=None, workspace=None, stream=None):
+        """Causal attention of a prompt chunk q ([T][q_heads][head_dim] fp16, row-strided) at context.., appended
+        before."""
+        import torch
+
+        t, qh, stride = self._check_q(q, context)
+        if out is None:
+            out = torch.empty((t, qh, self.head_dim), dtype=torch.float16, device=q.device)
+        if t == 0:
+            return out
+        if workspace is None:
+            workspace = torch.empty(lib().lfm3a_kv8_prefill_workspace_bytes(ctypes.byref(self.layout), t, qh,
+                                                                            context + t), dtype=torch.uint8,
+                                    device=q.device)
+        _check(lib().lfm3a_kv8_prefill(self._view, _ptr(q), stride, t, qh, context, self.sealed_below(context + t), window,
+                                       _ptr(out), _ptr(workspace), workspace.numel(), _stream(stream)))
+        return out
+
+    def key_weights(self, q, lse, ctx_len: int, window: int = 0, prev=None, decay: float = 1.0, out=None, stream=None):
+        """fp32 [kv_heads][ctx_len + m]: decay * prev plus the attention weight each key got from the m tokens of q,
+        summed over the query heads of its kv head. lse: of verify for the same q."""
+        import torch
+
+        m, qh, stride = self._check_q(q, ctx_len)
+        if lse.dtype != torch.float32 or tuple(lse.shape) != (m, qh) or not lse.is_contiguous():
+            raise LFM3AError(EINVAL, "lse must be fp32 [m][q_heads]")
+        n = ctx_len + m
+        if out is None:
+            out = torch.empty((self.kv_heads, n), dtype=torch.float32, device=q.device)
+        for t in (out, prev):
+            if t is not None and (t.dtype != torch.float32 or t.shape[0] != self.kv_heads or t.stride(1) != 1):
+                raise LFM3AError(EINVAL, "weights must be fp32 [kv_heads][>= ctx_len + m]")
+        _check(lib().lfm3a_kv8_weights(self._view, _ptr(q), stride, m, qh, ctx_len, self.sealed_below(n), window,
+                                       _ptr(lse), _ptr(prev), 0 if prev is None else prev.stride(0), decay, _ptr(out),
+                                       out.stride(0), _stream(stream)))
+        return out
+
+    def evict(self, weights, budget: int, sink: int, recent: int, dst: "LayerCache8", stream=None):
+        """Keeps `budget` tokens of each kv head (the first `sink`, the last `recent`, the heaviest others by
+        weights [kv_heads][>= length]) and moves them into dst, whose earlier content is replaced. Returns
+        (keep int32 [kv_heads][budget], the kept keys' weights)."""
+        if dst is self or budget > dst.capacity:
+            raise LFM3AError(EINVAL, "eviction needs another cache with room for the budget")
+        keep, kept = evict_select(weights, self.length, budget, sink, recent, stream=stream)
+        _check(lib().lfm3a_kv8_compact(self._view, self.length, self.sealed, _ptr(keep), budget, dst._view,
+                                       _stream(stream)))
+        dst.length, dst.sealed = budget, budget // BLOCK_TOKENS * BLOCK_TOKENS
+        return keep, kept
+
+
+def evict_select(weights, length: int, budget: int, sink: int, recent: int, stream=None):
+    """(keep int32 [kv_heads][budget] ascending, the kept keys' weights fp32) of weights fp32 [kv_heads][>= length]."""
+    import torch
+
+    h = weights.shape[0]
+    if weights.dtype != torch.float32 or weights.shape[1] < length or weights.stride(1) != 1:
+        raise LFM3AError(EINVAL, "weights must be fp32 [kv_heads][>= length]")
+    keep = torch.empty((h, max(0, budget)), dtype=torch.int32, device=weights.device)
+    kept = torch.empty((h, max(0, budget)), dtype=torch.float32, device=weights.device)
+    _check(lib().lfm3a_evict_select(_ptr(weights), weights.stride(0), h, length, sink, recent, budget, _ptr(keep),
+                                    _ptr(kept), kept.stride(0), _stream(stream)))
+    return keep, kept
 
 
 class PrefixCache:
