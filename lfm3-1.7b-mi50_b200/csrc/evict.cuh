@@ -7,12 +7,15 @@
 
 namespace lfm3a {
 
+// Keys of a block's share kept in shared memory; a longer share is read from global memory (L2) on every pass.
+constexpr int kEvictCache = 48 * 1024;
 struct EvictArgs {
   const float* w;        // [kv_heads][stride]
   int32_t* keep;         // [kv_heads][budget], ascending
   float* w_out;          // [kv_heads][out_stride] weights of the kept keys, or null
   int64_t stride, out_stride;
   int len, sink, recent, budget;
+  int cached;            // the blocks' shares fit kEvictCache
 };
 
 constexpr int kEvictCluster = 8, kEvictThreads = 1024;
@@ -36,6 +39,8 @@ __global__ __cluster_dims__(kEvictCluster, 1, 1) __launch_bounds__(kEvictThreads
   __shared__ uint32_t digit, above;
   __shared__ uint32_t counts[2];       // this block's keys above the threshold, and equal to it
   __shared__ uint32_t warp_sum[32];
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint32_t* keys = reinterpret_cast<uint32_t*>(smem);
   cg::cluster_group cluster = cg::this_cluster();
   pdl_wait();
   pdl_trigger();
@@ -47,6 +52,12 @@ __global__ __cluster_dims__(kEvictCluster, 1, 1) __launch_bounds__(kEvictThreads
   const int i0 = a.sink + (int)((int64_t)n * rank / kEvictCluster);
   const int i1 = a.sink + (int)((int64_t)n * (rank + 1) / kEvictCluster);
 
+  // A thread only ever looks at the keys it put there itself.
+  if (a.cached) {
+#pragma unroll 8
+    for (int i = i0 + tid; i < i1; i += kEvictThreads) keys[i - i0] = weight_key(w[i]);
+  }
+  auto key_at = [&](int i) { return a.cached ? keys[i - i0] : weight_key(w[i]); };
   uint32_t prefix = 0, mask = 0;      // digits found so far
   int left = k;                       // how many of the keys that match the prefix stay
   if (k > 0 && k < n) {               // the same in every thread of the cluster
@@ -54,8 +65,9 @@ __global__ __cluster_dims__(kEvictCluster, 1, 1) __launch_bounds__(kEvictThreads
       uint32_t* mine = hist[pass & 1];
       if (tid < 256) mine[tid] = 0;
       __syncthreads();
+#pragma unroll 4
       for (int i = i0 + tid; i < i1; i += kEvictThreads) {
-        const uint32_t key = weight_key(w[i]);
+        const uint32_t key = key_at(i);
         if ((key & mask) == prefix) atomicAdd(&mine[(key >> shift) & 255u], 1u);
       }
       cluster.sync();
@@ -107,8 +119,9 @@ __global__ __cluster_dims__(kEvictCluster, 1, 1) __launch_bounds__(kEvictThreads
   __syncthreads();
   uint32_t gt = 0, eq = 0;
   if (k > 0)
+#pragma unroll 4
     for (int i = i0 + tid; i < i1; i += kEvictThreads) {
-      const uint32_t key = weight_key(w[i]);
+      const uint32_t key = key_at(i);
       gt += all || key > prefix;
       eq += !all && key == prefix;
     }
@@ -145,11 +158,9 @@ __global__ __cluster_dims__(kEvictCluster, 1, 1) __launch_bounds__(kEvictThreads
   // In order, 1024 positions at a time: (above, equal) counts of the lanes before as one packed prefix sum.
   for (int base = i0; base < i1; base += kEvictThreads) {
     const int i = base + tid;
-    float wi = 0.f;
     bool is_gt = false, is_eq = false;
     if (i < i1) {
-      wi = w[i];
-      const uint32_t key = weight_key(wi);
+      const uint32_t key = key_at(i);
       is_gt = all || key > prefix;
       is_eq = !all && key == prefix;
     }
@@ -175,7 +186,7 @@ __global__ __cluster_dims__(kEvictCluster, 1, 1) __launch_bounds__(kEvictThreads
     if (is_gt || (is_eq && my_eq < (uint32_t)left)) {
       const int at = a.sink + (int)(my_gt + min(my_eq, (uint32_t)left));
       keep[at] = i;
-      if (w_out) w_out[at] = wi;
+      if (w_out) w_out[at] = w[i];
     }
     const uint32_t t = total[0];
     gt0 += t & 0xffffu;
@@ -194,67 +205,98 @@ struct Kv8CompactArgs {
 
 // One block per (page of the smaller cache, kv head): the values of its 32 kept tokens (fp32: code times scale, or the
 // tail's fp16) are sealed anew under their own scale; an incomplete last page goes to the smaller cache's tail in fp16.
+// A token's K is one contiguous run of its section, its V one byte in each word of D / 4 chunks; a thread has all its
+// loads in flight at once (taken one after the other, their latency was the whole time).
 template <int D, bool E4M3>
 __global__ __launch_bounds__(kSealThreads) void kv8_compact_kernel(Kv8CompactArgs a) {
   using S = Q8Section<D>;
-  constexpr int RS = kSealRow<D>;
-  __shared__ float x[2 * 32 * RS];
+  constexpr int RS = kSealRow<D>, KI = 2 * D / kSealThreads > 0 ? 2 * D / kSealThreads : 1, VI = 8 * D / kSealThreads;
+  __shared__ __align__(16) float x[2 * 32 * RS];
+  __shared__ __align__(16) uint8_t codes[32 * D];
   __shared__ float red[16];
   __shared__ const char* sec[32];
   __shared__ int pos[32];
+  __shared__ float2 scales[32];
   pdl_wait();
   pdl_trigger();
   const int tid = threadIdx.x, page = blockIdx.x, h = blockIdx.y, t0 = page * kBlockTokens;
   const int live = min(kBlockTokens, a.budget - t0);
-  const bool sealing = live == kBlockTokens;
   if (tid < live) {
     const int p = min(max(a.keep[(int64_t)h * a.budget + t0 + tid], 0), a.len - 1);
     pos[tid] = p;
-    sec[tid] = p < a.sealed ? a.src.pool + phys_block(a.src, p / kBlockTokens) * a.src.block_bytes + h * a.src.head_bytes
-                            : nullptr;
+    const char* s = nullptr;
+    if (p < a.sealed) {
+      s = a.src.pool + phys_block(a.src, p / kBlockTokens) * a.src.block_bytes + h * a.src.head_bytes;
+      const float2 f = *reinterpret_cast<const float2*>(s);
+      scales[tid] = make_float2(f.x * kCodeUnit<E4M3>, f.y * kCodeUnit<E4M3>);
+    }
+    sec[tid] = s;
   }
   __syncthreads();
   const TailView from = tail_of(a.src_tail, a.src.kv_heads, h, D);
-  for (int i = tid; i < live * (D / 16); i += kSealThreads) {   // 16 dims of one token's K
-    const int t = i / (D / 16), d0 = (i % (D / 16)) * 16, p = pos[t];
+  float kmax = 0.f, vmax = 0.f;
+  uint4 kr[KI], vr[VI];   // 16 dims of one token's K; 4 dims of one token's V (a byte of each word)
+#pragma unroll
+  for (int u = 0; u < KI; ++u) {
+    const int i = tid + u * kSealThreads, t = i / (D / 16), d0 = (i % (D / 16)) * 16;
+    kr[u] = make_uint4(0, 0, 0, 0);
+    if (i < 2 * D && t < live && sec[t])
+      kr[u] = *reinterpret_cast<const uint4*>(sec[t] + S::kOffK + S::k_chunk(pos[t] % kBlockTokens, d0) * 16);
+  }
+#pragma unroll
+  for (int u = 0; u < VI; ++u) {
+    const int i = tid + u * kSealThreads, t = i / (D / 4), k = i % (D / 4);   // chunk (dim pair of tiles k / 8, g = k % 8)
+    vr[u] = make_uint4(0, 0, 0, 0);
+    if (t < live && sec[t])
+      vr[u] = *reinterpret_cast<const uint4*>(sec[t] + S::kOffV + S::v_index(pos[t] % kBlockTokens & ~9, 32 * (k >> 3) + (k & 7)));
+  }
+#pragma unroll
+  for (int u = 0; u < KI; ++u) {
+    const int i = tid + u * kSealThreads, t = i / (D / 16), d0 = (i % (D / 16)) * 16;
+    if (i >= 2 * D || t >= live) continue;
     float* row = x + t * RS + d0;
     if (sec[t]) {
-      const float ks = reinterpret_cast<const float*>(sec[t])[0];
-      const uint4 r = *reinterpret_cast<const uint4*>(sec[t] + S::kOffK + S::k_chunk(p % kBlockTokens, d0) * 16);
-      const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+      const float ks = scales[t].x;
+      const uint32_t w[4] = {kr[u].x, kr[u].y, kr[u].z, kr[u].w};
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const float2 lo = unpack_half2(decode_pair<E4M3, false>(w[k])), hi = unpack_half2(decode_pair<E4M3, true>(w[k]));
-        row[4 * k] = lo.x * kCodeUnit<E4M3> * ks;
-        row[4 * k + 1] = lo.y * kCodeUnit<E4M3> * ks;
-        row[4 * k + 2] = hi.x * kCodeUnit<E4M3> * ks;
-        row[4 * k + 3] = hi.y * kCodeUnit<E4M3> * ks;
+        const float2 p = unpack_half2(decode_pair<E4M3, false>(w[k])), q = unpack_half2(decode_pair<E4M3, true>(w[k]));
+        const float4 f = make_float4(p.x * ks, p.y * ks, q.x * ks, q.y * ks);
+        *reinterpret_cast<float4*>(row + 4 * k) = f;
+        kmax = fmaxf(kmax, fmaxf(fmaxf(fabsf(f.x), fabsf(f.y)), fmaxf(fabsf(f.z), fabsf(f.w))));
       }
     } else {
-#pragma unroll
-      for (int k = 0; k < 16; ++k) row[k] = __half2float(from.k[(int64_t)(p % kTailTokens) * D + d0 + k]);
+      const __half* src = from.k + (int64_t)(pos[t] % kTailTokens) * D + d0;
+      kmax = fmaxf(kmax, stage_row8(src, true, row));
+      kmax = fmaxf(kmax, stage_row8(src + 8, true, row + 8));
     }
   }
-  for (int i = tid; i < live * D; i += kSealThreads) {
-    const int t = i / D, d = i % D, p = pos[t];
-    float v;
-    if (sec[t])
-      v = decode8<E4M3>((uint8_t)sec[t][S::kOffV + S::v_index(p % kBlockTokens, d)]) *
-          reinterpret_cast<const float*>(sec[t])[1];
-    else
-      v = __half2float(from.v[(int64_t)d * kTailTokens + p % kTailTokens]);
-    x[32 * RS + t * RS + d] = v;
+#pragma unroll
+  for (int u = 0; u < VI; ++u) {
+    const int i = tid + u * kSealThreads, t = i / (D / 4), k = i % (D / 4), d0 = 32 * (k >> 3) + (k & 7);
+    if (t >= live) continue;
+    const int p = pos[t], byte = (p >> 3 & 1) * 2 + (p & 1);
+    const uint32_t w[4] = {vr[u].x, vr[u].y, vr[u].z, vr[u].w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int d = d0 + 8 * e;
+      float f;
+      if (sec[t]) f = unpack_half2(decode_pair<E4M3, false>(w[e] >> (8 * byte) & 0xffu)).x * scales[t].y;
+      else f = __half2float(from.v[(int64_t)d * kTailTokens + p % kTailTokens]);
+      x[(32 + t) * RS + d] = f;
+      vmax = fmaxf(vmax, fabsf(f));
+    }
   }
-  __syncthreads();
-  if (sealing) {
-    seal_page<D, E4M3>(x, red, a.dst.pool + phys_block(a.dst, page) * a.dst.block_bytes + h * a.dst.head_bytes);
+  if (live == kBlockTokens) {
+    seal_page<D, E4M3>(x, kmax, vmax, red, codes, a.dst.pool + phys_block(a.dst, page) * a.dst.block_bytes + h * a.dst.head_bytes);
     return;
   }
+  __syncthreads();
   const TailView to = tail_of(a.dst_tail, a.dst.kv_heads, h, D);
   for (int i = tid; i < live * D; i += kSealThreads) {
     const int t = i / D, d = i % D, slot = (t0 + t) % kTailTokens;
     to.k[(int64_t)slot * D + d] = __float2half_rn(x[t * RS + d]);
-    to.v[(int64_t)d * kTailTokens + slot] = __float2half_rn(x[32 * RS + t * RS + d]);
+    to.v[(int64_t)d * kTailTokens + slot] = __float2half_rn(x[(32 + t) * RS + d]);
   }
 }
 

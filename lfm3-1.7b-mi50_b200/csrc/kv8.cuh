@@ -53,16 +53,23 @@ __host__ __device__ __forceinline__ TailView tail_of(__half* tail, int kv_heads,
 // fp16 values of the cache are finite: NaN becomes 0, an infinity the largest finite value of its sign.
 __device__ __forceinline__ float finite_f16(float x) { return x != x ? 0.f : fminf(fmaxf(x, -65504.f), 65504.f); }
 
-// The 8-bit code of x / scale and the value a code stands for (before the scale).
+// The 8-bit code of the fp32 quotient x / scale, to nearest even (inv: the rounded reciprocal of scale, |x| at most 127
+// or 448 scales). x * inv is within 2^-22 of the quotient, relatively, so it decides the code unless a rounding boundary
+// lies that near; then the division itself does. (Dividing every value took half of the append kernel's time.)
 template <bool E4M3>
-__device__ __forceinline__ uint32_t encode8(float x, float scale) {
-  const float y = __fdiv_rn(x, scale);
-  if (E4M3) {   // round to nearest even, saturating at 448
+__device__ __forceinline__ uint32_t encode8(float x, float scale, float inv) {
+  if (E4M3) {   // saturating at 448
+    const float y = x * inv;
     uint16_t r;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(0.f), "f"(y));
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(y * (1.f + 0x1p-21f)), "f"(y * (1.f - 0x1p-21f)));
+    if ((r >> 8) != (r & 0xffu))
+      asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(0.f), "f"(__fdiv_rn(x, scale)));
     return (uint32_t)r & 0xffu;
   }
-  return (uint32_t)__float2int_rn(fminf(fmaxf(y, -127.f), 127.f)) & 0xffu;
+  constexpr float kMagic = 12582912.f;   // 1.5 * 2^23: adding it rounds to an integer, whose low byte is the code
+  float t = fmaf(x, inv, kMagic);
+  if (fabsf(fmaf(x, inv, kMagic - t)) > 0.4999f) t = __fdiv_rn(x, scale) + kMagic;
+  return __float_as_uint(t) & 0xffu;
 }
 
 // Bytes 0, 1 (LO) or 2, 3 of a word of codes as an fp16 pair. int8: 0x64NN is 1024 + NN with NN = v ^ 0x80, minus
@@ -96,63 +103,97 @@ __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
 }
 
 // ---------------------------------------------------------------- append and sealing
-// Seals one page and kv head from fp32 rows in shared memory (x [2][32][D + 1]: K, then V; the odd row stride keeps the
-// V chunks' walk over dims free of bank conflicts), by 256 threads.
+// Seals one page and kv head from fp32 rows in shared memory (x [2][32][kSealRow]: K, then V), by 256 threads, each with
+// the largest magnitude of the K and V values it put there. codes: 32 D bytes of shared memory. A thread makes 16 codes
+// at a time: a whole 16-byte chunk of K, which goes out as it is, or 4 dims x 4 keys of V, four words of four chunks,
+// which are put in order in shared memory first.
 constexpr int kSealThreads = 256;
 template <int D>
-constexpr int kSealRow = D + 1;
+constexpr int kSealRow = D + 4;   // floats; 16-byte aligned rows
 template <int D, bool E4M3>
-__device__ __forceinline__ void seal_page(const float* x, float* red, char* sec) {
+__device__ __forceinline__ void seal_page(const float* x, float kmax, float vmax, float* red, uint8_t* codes, char* sec) {
   using S = Q8Section<D>;
   constexpr int RS = kSealRow<D>;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  float scale[2];
 #pragma unroll
-  for (int s = 0; s < 2; ++s) {
-    const float* xs = x + s * 32 * RS;
-    float amax = 0.f;
-    for (int i = tid; i < 32 * D; i += kSealThreads) amax = fmaxf(amax, fabsf(xs[(i / D) * RS + i % D]));
-#pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    if (lane == 0) red[8 * s + warp] = amax;
+  for (int o = 16; o >= 1; o >>= 1) {
+    kmax = fmaxf(kmax, __shfl_xor_sync(0xffffffffu, kmax, o));
+    vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, o));
   }
-  __syncthreads();
+  if (lane == 0) {
+    red[warp] = kmax;
+    red[8 + warp] = vmax;
+  }
+  __syncthreads();   // also publishes x
+  float scale[2], inv[2];
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
     float amax = red[8 * s];
 #pragma unroll
     for (int w = 1; w < 8; ++w) amax = fmaxf(amax, red[8 * s + w]);
     scale[s] = amax > 0.f ? __fdiv_rn(amax, E4M3 ? 448.f : 127.f) : 1.f;
+    inv[s] = __fdiv_rn(1.f, scale[s]);
   }
   if (tid < 8) reinterpret_cast<float*>(sec)[tid] = tid < 2 ? scale[tid] : 0.f;
   uint4* K = reinterpret_cast<uint4*>(sec + S::kOffK);
-  uint4* V = reinterpret_cast<uint4*>(sec + S::kOffV);
-  for (int i = tid; i < 2 * D; i += kSealThreads) {   // 16-byte chunks of K: 16 dims of one key
-    const int l = i & 31, a = i >> 5;
-    const int key = (a / (D / 64)) * 8 + (l >> 2), dim0 = (a % (D / 64)) * 64 + (l & 3) * 16;
-    uint32_t w[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      w[k] = 0;
-#pragma unroll
-      for (int b = 0; b < 4; ++b) w[k] |= encode8<E4M3>(x[key * RS + dim0 + 4 * k + b], scale[0]) << (8 * b);
-    }
-    K[i] = make_uint4(w[0], w[1], w[2], w[3]);
-  }
   const float* v = x + 32 * RS;
-  for (int i = tid; i < 2 * D; i += kSealThreads) {   // of V: four dims of four keys
-    const int l = i & 31, a = i >> 5;
-    const int key0 = (a / (D / 32)) * 16 + (l & 3) * 2, dim0 = (a % (D / 32)) * 32 + (l >> 2);
-    uint32_t w[4];
+  for (int i = tid; i < 4 * D; i += kSealThreads) {
+    if (i < 2 * D) {   // 16 dims of one key
+      const int l = i & 31, a = i >> 5;
+      const int key = (a / (D / 64)) * 8 + (l >> 2), dim0 = (a % (D / 64)) * 64 + (l & 3) * 16;
+      uint32_t w[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      w[k] = 0;
+      for (int k = 0; k < 4; ++k) {
+        const float4 f = *reinterpret_cast<const float4*>(x + key * RS + dim0 + 4 * k);
+        w[k] = encode8<E4M3>(f.x, scale[0], inv[0]) | encode8<E4M3>(f.y, scale[0], inv[0]) << 8 |
+               encode8<E4M3>(f.z, scale[0], inv[0]) << 16 | encode8<E4M3>(f.w, scale[0], inv[0]) << 24;
+      }
+      K[i] = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {           // dims dim0 .. + 3 of keys key0, + 1, + 8, + 9
+      const int k = i - 2 * D, c = k & 3, wi = (k >> 2) & 3, gh = (k >> 4) & 1, dtp = (k >> 5) % (D / 32), mt = (k >> 5) / (D / 32);
+      const int key0 = 16 * mt + 2 * c, dim0 = 32 * dtp + 16 * (wi >> 1) + 8 * (wi & 1) + 4 * gh;
+      uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
-      for (int b = 0; b < 4; ++b)
-        w[k] |= encode8<E4M3>(v[(key0 + (b & 1) + 8 * (b >> 1)) * RS + dim0 + 8 * k], scale[1]) << (8 * b);
+      for (int b = 0; b < 4; ++b) {
+        const float4 f = *reinterpret_cast<const float4*>(v + (key0 + (b & 1) + 8 * (b >> 1)) * RS + dim0);
+        w[0] |= encode8<E4M3>(f.x, scale[1], inv[1]) << (8 * b);
+        w[1] |= encode8<E4M3>(f.y, scale[1], inv[1]) << (8 * b);
+        w[2] |= encode8<E4M3>(f.z, scale[1], inv[1]) << (8 * b);
+        w[3] |= encode8<E4M3>(f.w, scale[1], inv[1]) << (8 * b);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) *reinterpret_cast<uint32_t*>(codes + S::v_index(key0, dim0 + e)) = w[e];
     }
-    V[i] = make_uint4(w[0], w[1], w[2], w[3]);
   }
+  __syncthreads();
+  uint4* V = reinterpret_cast<uint4*>(sec + S::kOffV);
+  for (int i = tid; i < 2 * D; i += kSealThreads) V[i] = reinterpret_cast<const uint4*>(codes)[i];
+}
+
+__device__ __forceinline__ void unpack_row8(uint4 v, float (&f)[8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 p = unpack_half2(w[i]);
+    f[2 * i] = finite_f16(p.x);
+    f[2 * i + 1] = finite_f16(p.y);
+  }
+}
+// 8 halves at p (16-byte aligned when vec) as finite floats into dst (16-byte aligned); returns their largest magnitude.
+__device__ __forceinline__ float stage_row8(const __half* p, bool vec, float* dst) {
+  float f[8];
+  if (vec) {
+    unpack_row8(*reinterpret_cast<const uint4*>(p), f);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = finite_f16(__half2float(p[i]));
+  }
+  *reinterpret_cast<float4*>(dst) = make_float4(f[0], f[1], f[2], f[3]);
+  *reinterpret_cast<float4*>(dst + 4) = make_float4(f[4], f[5], f[6], f[7]);
+  float m = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(f[i]));
+  return m;
 }
 
 struct Kv8AppendArgs {
@@ -160,61 +201,80 @@ struct Kv8AppendArgs {
   __half* tail;
   int page0;         // first page of the launch
   int seal_page_end; // pages below are sealed, the others go to the tail
+  int vec;           // rows of k and v start 16-byte aligned
 };
 
-// One block per (page, kv head): the page's tokens below pos0 come from the tail, the others from the new rows. Bound
-// by memory for prompt chunks, by latency for drafts; the fp16 K is the one lfm3a_kv_append stores.
+// One block per (page, kv head): the page's tokens below pos0 come from the tail, the others from the new rows (8 values
+// a load; K through the fp16 k-norm and RoPE that lfm3a_kv_append applies). Bound by memory for prompt chunks, by the
+// latency of one round of loads for drafts.
 template <int D, bool E4M3>
 __global__ __launch_bounds__(kSealThreads) void kv8_append_kernel(Kv8AppendArgs args) {
-  constexpr int J = D / 64, HALF = D / 2, RS = kSealRow<D>;
-  __shared__ float x[2 * 32 * RS];
+  constexpr int J = D / 64, HALF = D / 2, RS = kSealRow<D>, R8 = D / 8;
+  __shared__ __align__(16) float x[2 * 32 * RS];
+  __shared__ __align__(16) uint8_t codes[32 * D];
   __shared__ float red[16];
   pdl_wait();
   pdl_trigger();
   const AppendArgs& a = args.a;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int page = args.page0 + blockIdx.x, h = blockIdx.y, t0 = page * kBlockTokens;
-  const int end = min(t0 + kBlockTokens, a.pos0 + a.n);
-  const bool sealing = page < args.seal_page_end;
+  const int lo = max(t0, a.pos0), end = min(t0 + kBlockTokens, a.pos0 + a.n);   // new tokens
+  const bool sealing = page < args.seal_page_end, vec = args.vec != 0, plain = !a.knorm && !a.rope;
+  if (!sealing && lo >= end) return;
   const TailView tail = tail_of(args.tail, a.g.kv_heads, h, D);
-  if (sealing) {
-    const int old = min(a.pos0, t0 + kBlockTokens) - t0;   // tokens that wait in the tail
-    for (int i = tid; i < old * D; i += kSealThreads) {
-      const int t = i / D, d = i % D;
-      x[t * RS + d] = __half2float(tail.k[(int64_t)((t0 + t) % kTailTokens) * D + d]);
-    }
-    for (int i = tid; i < kBlockTokens * D; i += kSealThreads) {
-      const int t = i & 31, d = i >> 5;
-      if (t < old) x[32 * RS + t * RS + d] = __half2float(tail.v[d * kTailTokens + (t0 + t) % kTailTokens]);
-    }
-  }
-  for (int t = max(t0, a.pos0) + warp; t < end; t += 8) {
-    const int i = t - a.pos0, r = t - t0, slot = t % kTailTokens;
-    const __half* ks = a.k + (int64_t)i * a.stride + h * D;
-    const __half* vs = a.v + (int64_t)i * a.stride + h * D;
-    float ra[J], rb[J];
-    norm_rope_pairs<D>(a, ks, t, lane, ra, rb);
+  float kmax = 0.f, vmax = 0.f;
 #pragma unroll
-    for (int j = 0; j < J; ++j) {
-      const int d0 = lane + 32 * j, d1 = d0 + HALF;
-      const float k0 = finite_f16(ra[j]), k1 = finite_f16(rb[j]);
-      const float v0 = finite_f16(__half2float(vs[d0])), v1 = finite_f16(__half2float(vs[d1]));
-      if (sealing) {
-        x[r * RS + d0] = k0;
-        x[r * RS + d1] = k1;
-        x[32 * RS + r * RS + d0] = v0;
-        x[32 * RS + r * RS + d1] = v1;
-      } else {
-        tail.k[(int64_t)slot * D + d0] = __float2half_rn(k0);
-        tail.k[(int64_t)slot * D + d1] = __float2half_rn(k1);
-        tail.v[d0 * kTailTokens + slot] = __float2half_rn(v0);
-        tail.v[d1 * kTailTokens + slot] = __float2half_rn(v1);
+  for (int i = tid; i < kBlockTokens * R8; i += kSealThreads) {
+    const int r = i / R8, d = (i % R8) * 8, t = t0 + r;
+    if (t < lo || t >= end) continue;
+    const int64_t at = (int64_t)(t - a.pos0) * a.stride + h * D + d;
+    if (plain) kmax = fmaxf(kmax, stage_row8(a.k + at, vec, x + r * RS + d));
+    vmax = fmaxf(vmax, stage_row8(a.v + at, vec, x + (32 + r) * RS + d));
+  }
+  if (!plain) {
+#pragma unroll 4
+    for (int t = lo + warp; t < end; t += 8) {
+      float ra[J], rb[J];
+      norm_rope_pairs<D>(a, a.k + (int64_t)(t - a.pos0) * a.stride + h * D, t, lane, ra, rb);
+      float* row = x + (t - t0) * RS;
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        const float k0 = finite_f16(ra[j]), k1 = finite_f16(rb[j]);
+        row[lane + 32 * j] = k0;
+        row[lane + 32 * j + HALF] = k1;
+        kmax = fmaxf(kmax, fmaxf(fabsf(k0), fabsf(k1)));
       }
     }
   }
-  if (!sealing) return;
-  __syncthreads();
-  seal_page<D, E4M3>(x, red, a.g.pool + phys_block(a.g, page) * a.g.block_bytes + h * a.g.head_bytes);
+  if (!sealing) {
+    __syncthreads();
+    for (int i = tid; i < (end - lo) * D; i += kSealThreads) {
+      const int t = lo + i / D, d = i % D, slot = t % kTailTokens;
+      tail.k[(int64_t)slot * D + d] = __float2half_rn(x[(t - t0) * RS + d]);
+      tail.v[(int64_t)d * kTailTokens + slot] = __float2half_rn(x[(32 + t - t0) * RS + d]);
+    }
+    return;
+  }
+  if (lo > t0) {   // tokens that wait in the tail
+    const int old = min(lo, t0 + kBlockTokens) - t0, slot0 = t0 % kTailTokens;
+    for (int i = tid; i < old * R8; i += kSealThreads) {
+      const int r = i / R8, d = (i % R8) * 8;
+      kmax = fmaxf(kmax, stage_row8(tail.k + (int64_t)(slot0 + r) * D + d, true, x + r * RS + d));
+    }
+    for (int i = tid; i < D * 4; i += kSealThreads) {   // 8 tokens of one dim
+      const int d = i >> 2, r0 = (i & 3) * 8;
+      if (r0 >= old) continue;
+      float f[8];
+      unpack_row8(*reinterpret_cast<const uint4*>(tail.v + (int64_t)d * kTailTokens + slot0 + r0), f);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (r0 + e < old) {
+          x[(32 + r0 + e) * RS + d] = f[e];
+          vmax = fmaxf(vmax, fabsf(f[e]));
+        }
+    }
+  }
+  seal_page<D, E4M3>(x, kmax, vmax, red, codes, a.g.pool + phys_block(a.g, page) * a.g.block_bytes + h * a.g.head_bytes);
 }
 
 // ---------------------------------------------------------------- reading back
@@ -226,37 +286,73 @@ struct Kv8ReadArgs {
   int pos0, n, sealed;
 };
 
-// One block per (page, kv head): the values the cache stands for, rounded to fp16.
+// One block per (page, kv head): the values the cache stands for, rounded to fp16; 16-byte stores of 8 dims of a token.
 template <int D, bool E4M3>
-__global__ __launch_bounds__(256) void kv8_read_kernel(Kv8ReadArgs a) {
+__global__ __launch_bounds__(128) void kv8_read_kernel(Kv8ReadArgs a) {
   using S = Q8Section<D>;
   pdl_wait();
   pdl_trigger();
   const int tid = threadIdx.x, page = a.pos0 / kBlockTokens + blockIdx.x, h = blockIdx.y, t0 = page * kBlockTokens;
   const int lo = max(a.pos0, t0), hi = min(a.pos0 + a.n, t0 + kBlockTokens);
   const int64_t row = (int64_t)a.g.kv_heads * D;
+  __half* const k_out = a.k + h * D;
+  __half* const v_out = a.v + h * D;
   if (t0 < a.sealed) {
     const char* sec = a.g.pool + phys_block(a.g, page) * a.g.block_bytes + h * a.g.head_bytes;
-    const float ks = reinterpret_cast<const float*>(sec)[0], vs = reinterpret_cast<const float*>(sec)[1];
-    for (int i = tid; i < 32 * (D / 2); i += 256) {   // pairs of dims
-      const int t = i / (D / 2), d = 2 * (i % (D / 2));
-      if (t0 + t < lo || t0 + t >= hi) continue;
-      const int64_t at = (t0 + t - a.pos0) * row + h * D + d;
-      const uint32_t kk = *reinterpret_cast<const uint16_t*>(sec + S::kOffK + S::k_chunk(t, d) * 16 + (d & 15));
-      const uint32_t v0 = (uint8_t)sec[S::kOffV + S::v_index(t, d)], v1 = (uint8_t)sec[S::kOffV + S::v_index(t, d + 1)];
-      const float2 kf = unpack_half2(decode_pair<E4M3, false>(kk));
-      *reinterpret_cast<uint32_t*>(a.k + at) =
-          pack_half2(kf.x * kCodeUnit<E4M3> * ks, kf.y * kCodeUnit<E4M3> * ks);
-      *reinterpret_cast<uint32_t*>(a.v + at) = pack_half2(decode8<E4M3>(v0) * vs, decode8<E4M3>(v1) * vs);
+    const float ks = reinterpret_cast<const float*>(sec)[0] * kCodeUnit<E4M3>;
+    const float vs = reinterpret_cast<const float*>(sec)[1] * kCodeUnit<E4M3>;
+    const uint4* K = reinterpret_cast<const uint4*>(sec + S::kOffK);
+    const uint32_t* V = reinterpret_cast<const uint32_t*>(sec + S::kOffV);
+#pragma unroll
+    for (int i = tid; i < 2 * D; i += 128) {   // 16 dims of one key
+      const int l = i & 31, s = i >> 5;
+      const int t = t0 + (s / (D / 64)) * 8 + (l >> 2), d = (s % (D / 64)) * 64 + (l & 3) * 16;
+      const uint4 r = K[i];
+      const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+      uint32_t o[8];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 p = unpack_half2(decode_pair<E4M3, false>(w[k])), q = unpack_half2(decode_pair<E4M3, true>(w[k]));
+        o[2 * k] = pack_half2(p.x * ks, p.y * ks);
+        o[2 * k + 1] = pack_half2(q.x * ks, q.y * ks);
+      }
+      if (t < lo || t >= hi) continue;
+      uint4* dst = reinterpret_cast<uint4*>(k_out + (t - a.pos0) * row + d);
+      dst[0] = make_uint4(o[0], o[1], o[2], o[3]);
+      dst[1] = make_uint4(o[4], o[5], o[6], o[7]);
+    }
+#pragma unroll
+    for (int i = tid; i < D; i += 128) {   // 8 dims (one word each) of keys key0, + 1, + 8, + 9
+      const int c = i & 3, wi = (i >> 2) & 3, dtp = (i >> 4) % (D / 32), mt = (i >> 4) / (D / 32);
+      const int key0 = 16 * mt + 2 * c, d = 32 * dtp + 16 * (wi >> 1) + 8 * (wi & 1);
+      uint32_t w[8];
+#pragma unroll
+      for (int g = 0; g < 8; ++g) w[g] = V[S::v_index(key0, d + g) / 4];
+      float f[4][8];
+#pragma unroll
+      for (int g = 0; g < 8; ++g) {
+        const float2 p = unpack_half2(decode_pair<E4M3, false>(w[g])), q = unpack_half2(decode_pair<E4M3, true>(w[g]));
+        f[0][g] = p.x * vs;
+        f[1][g] = p.y * vs;
+        f[2][g] = q.x * vs;
+        f[3][g] = q.y * vs;
+      }
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        const int t = t0 + key0 + (b & 1) + 8 * (b >> 1);
+        if (t < lo || t >= hi) continue;
+        *reinterpret_cast<uint4*>(v_out + (t - a.pos0) * row + d) =
+            make_uint4(pack_half2(f[b][0], f[b][1]), pack_half2(f[b][2], f[b][3]), pack_half2(f[b][4], f[b][5]),
+                       pack_half2(f[b][6], f[b][7]));
+      }
     }
   } else {
     const TailView tail = tail_of(a.tail, a.g.kv_heads, h, D);
-    for (int i = tid; i < 32 * D; i += 256) {
-      const int t = t0 + i / D, d = i % D, slot = t % kTailTokens;
-      if (t < lo || t >= hi) continue;
-      const int64_t at = (t - a.pos0) * row + h * D + d;
-      a.k[at] = tail.k[(int64_t)slot * D + d];
-      a.v[at] = tail.v[d * kTailTokens + slot];
+    for (int i = tid; i < (hi - lo) * D; i += 128) {
+      const int t = lo + i / D, d = i % D, slot = t % kTailTokens;
+      const int64_t at = (t - a.pos0) * row + d;
+      k_out[at] = tail.k[(int64_t)slot * D + d];
+      v_out[at] = tail.v[(int64_t)d * kTailTokens + slot];
     }
   }
 }
@@ -722,7 +818,7 @@ struct Kv8ExpandArgs {
 // One page and kv head of the cache as the K and V tiles of a MODE_F16 section, the codes as fp16 (exactly; the scales go
 // beside them): what the prefill kernel's SCALED form reads. Values past the sequence's end are 0.
 template <int D, bool E4M3>
-__global__ __launch_bounds__(256) void kv8_expand_kernel(Kv8ExpandArgs a) {
+__global__ __launch_bounds__(128) void kv8_expand_kernel(Kv8ExpandArgs a) {
   using S = Q8Section<D>;
   using F = F16Section<D>;
   pdl_wait();
@@ -740,25 +836,35 @@ __global__ __launch_bounds__(256) void kv8_expand_kernel(Kv8ExpandArgs a) {
       const float vs = reinterpret_cast<const float*>(sec)[1] * kCodeUnit<E4M3>;
       a.scales[section] = make_float4(ks, log2f(vs), 1.f / vs, 0.f);
     }
-    for (int i = tid; i < 4 * D; i += 256) {   // 16-byte rows of the tiles: 8 dims of one key, 8 keys of one dim
-      const int e = i & 7, tile = i >> 3;
-      const int key = (tile / (D / 8)) * 8 + e, d = (tile % (D / 8)) * 8;
-      const uint2 w = *reinterpret_cast<const uint2*>(sec + S::kOffK + S::k_chunk(key, d) * 16 + (d & 15));
-      K[i] = make_uint4(decode_pair<E4M3, false>(w.x), decode_pair<E4M3, true>(w.x), decode_pair<E4M3, false>(w.y),
-                        decode_pair<E4M3, true>(w.y));
-      const int vd = (tile >> 2) * 8 + e, key0 = (tile & 3) * 8;
-      uint32_t v[4];
+    // Tile rows of 16 bytes: 8 dims of one key (K), 8 keys of one dim (V).
+    for (int i = tid; i < 2 * D; i += 128) {
+      const int l = i & 31, b = i >> 5;
+      const int key = (b / (D / 64)) * 8 + (l >> 2), d8 = (b % (D / 64)) * 8 + (l & 3) * 2;
+      const uint4 w = reinterpret_cast<const uint4*>(sec + S::kOffK)[i];
+      uint4* dst = K + ((key >> 3) * (D / 8) + d8) * 8 + (key & 7);
+      dst[0] = make_uint4(decode_pair<E4M3, false>(w.x), decode_pair<E4M3, true>(w.x), decode_pair<E4M3, false>(w.y),
+                          decode_pair<E4M3, true>(w.y));
+      dst[8] = make_uint4(decode_pair<E4M3, false>(w.z), decode_pair<E4M3, true>(w.z), decode_pair<E4M3, false>(w.w),
+                          decode_pair<E4M3, true>(w.w));
+    }
+    const uint32_t* V4 = reinterpret_cast<const uint32_t*>(sec + S::kOffV);
+    for (int i = tid; i < 2 * D; i += 128) {   // 16 keys of one dim: four words
+      const int wi = i & 3, g = (i >> 2) & 7, dtp = (i >> 5) % (D / 32), mt = (i >> 5) / (D / 32);
+      const int d = 32 * dtp + 16 * (wi >> 1) + 8 * (wi & 1) + g;
+      uint32_t w[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k)   // keys key0 + 2 k and the next lie in neighbouring bytes
-        v[k] = decode_pair<E4M3, false>(
-            *reinterpret_cast<const uint16_t*>(sec + S::kOffV + S::v_index(key0 + 2 * k, vd)));
-      V[i] = make_uint4(v[0], v[1], v[2], v[3]);
+      for (int c = 0; c < 4; ++c) w[c] = V4[S::v_index(16 * mt + 2 * c, d) / 4];
+      uint4* dst = V + ((d >> 3) * 4 + 2 * mt) * 8 + (d & 7);
+      dst[0] = make_uint4(decode_pair<E4M3, false>(w[0]), decode_pair<E4M3, false>(w[1]), decode_pair<E4M3, false>(w[2]),
+                          decode_pair<E4M3, false>(w[3]));
+      dst[8] = make_uint4(decode_pair<E4M3, true>(w[0]), decode_pair<E4M3, true>(w[1]), decode_pair<E4M3, true>(w[2]),
+                          decode_pair<E4M3, true>(w[3]));
     }
     return;
   }
   const TailView tail = tail_of(a.tail, a.g.kv_heads, h, D);
   if (tid == 0) a.scales[section] = make_float4(1.f, 0.f, 1.f, 0.f);
-  for (int i = tid; i < 4 * D; i += 256) {
+  for (int i = tid; i < 4 * D; i += 128) {
     const int e = i & 7, tile = i >> 3;
     const int key = (tile / (D / 8)) * 8 + e, d = (tile % (D / 8)) * 8;
     K[i] = t0 + key < a.len ? *reinterpret_cast<const uint4*>(tail.k + (int64_t)((t0 + key) % kTailTokens) * D + d)
@@ -787,7 +893,7 @@ struct Kv8WeightArgs {
 
 template <int D>
 struct Kv8Weights {
-  static constexpr int kWarps = 8, kThreads = 32 * kWarps, kStages = 4;
+  static constexpr int kWarps = 8, kThreads = 32 * kWarps, kStages = D == 64 ? 4 : 2;
   static constexpr int kStageBytes = Q8Section<D>::kOffV;   // the header and K
   static constexpr int kRing = kWarps * kStages * kStageBytes;
   static constexpr int kMaxRows = 256;
@@ -797,11 +903,12 @@ struct Kv8Weights {
 };
 
 // out[h][key] = decay prev[h][key] + sum over the m tokens and the head's query rows of 2^(s - lse): only K is read. A
-// warp takes a page (as kv8_attend_kernel does), makes its K operands once and passes over the query rows 8 at a time;
-// a lane owns the weights of 4 keys for 2 rows in 8, so the sums meet in two shuffles at the end and no atomics are
-// needed. Grid (splits, kv heads).
+// warp takes a page (as kv8_attend_kernel does), makes its K operands once and passes over the query rows 8 at a time, two
+// independent chains of MMAs (16 keys each) per 8 rows; a lane owns the weights of 4 keys for 2 rows in 8, so the sums
+// meet in two shuffles per page and no atomics are needed. prev is loaded a page ahead (loaded when wanted, its latency
+// was two thirds of the time of a single token's pass). Grid (splits, kv heads).
 template <int D, bool E4M3>
-__global__ __launch_bounds__(Kv8Weights<D>::kThreads, D == 64 ? 2 : 1) void kv8_weights_kernel(Kv8WeightArgs a) {
+__global__ __launch_bounds__(Kv8Weights<D>::kThreads, 2) void kv8_weights_kernel(Kv8WeightArgs a) {
   using L = Kv8Weights<D>;
   using S = Q8Section<D>;
   constexpr int NE = D / 64, W = L::kWarps, NS = L::kStages;
@@ -841,44 +948,54 @@ __global__ __launch_bounds__(Kv8Weights<D>::kThreads, D == 64 ? 2 : 1) void kv8_
   __syncthreads();
 
   const TailView tail = tail_of(a.tail, a.g.kv_heads, h, D);
-  float w[2];   // keys key0 + g, key0 + g + 8
-  auto rows16 = [&](const uint32_t (&f)[4 * NE][4], int key0, bool open, float kc) {
-    w[0] = w[1] = 0.f;
+  // The page's 32 keys against all rows; lane i adds key i's sum to old and stores it.
+  auto rows32 = [&](const uint32_t (&f)[2][4 * NE][4], int page, bool open, float kc, float old) {
+    float w[4] = {0.f, 0.f, 0.f, 0.f};   // keys 8 i + g
 #pragma unroll 2
     for (int n = 0; n < ntiles; ++n) {
-      float s[4] = {0.f, 0.f, 0.f, 0.f};
+      float s[2][4] = {};
 #pragma unroll
       for (int e = 0; e < 2 * NE; ++e) {
         const uint4 qv = sq[(n * 2 * NE + e) * 32 + lane];
-        mma_f16_16816(s, f[2 * e], qv.x, qv.y);
-        mma_f16_16816(s, f[2 * e + 1], qv.z, qv.w);
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) mma_f16_16816(s[mt], f[mt][2 * e], qv.x, qv.y);
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) mma_f16_16816(s[mt], f[mt][2 * e + 1], qv.z, qv.w);
       }
       const float2 z = *reinterpret_cast<const float2*>(slse + 8 * n + 2 * c);
-      float p[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) p[i] = fast_exp2(fmaf(s[i], kc, (i & 1) ? -z.y : -z.x));
-      if (!open) {
+      for (int mt = 0; mt < 2; ++mt) {
+        float p[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int pos = a.ctx_len + (8 * n + 2 * c + (i & 1)) / a.group;
-          if (!sees(pos, key0 + g + 8 * (i >> 1), a.window)) p[i] = 0.f;
+        for (int i = 0; i < 4; ++i) p[i] = fast_exp2(fmaf(s[mt][i], kc, (i & 1) ? -z.y : -z.x));
+        if (!open) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int pos = a.ctx_len + (8 * n + 2 * c + (i & 1)) / a.group;
+            if (!sees(pos, page * kBlockTokens + 16 * mt + g + 8 * (i >> 1), a.window)) p[i] = 0.f;
+          }
         }
+        w[2 * mt] += p[0] + p[1];
+        w[2 * mt + 1] += p[2] + p[3];
       }
-      w[0] += p[0] + p[1];
-      w[1] += p[2] + p[3];
     }
+    float mine = 0.f;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < 4; ++i) {
       w[i] += __shfl_xor_sync(0xffffffffu, w[i], 1);
       w[i] += __shfl_xor_sync(0xffffffffu, w[i], 2);
-      const int key = key0 + g + 8 * i;
-      if (c == 0 && key < kv_end) {
-        const float old = a.prev ? a.decay * a.prev[h * a.prev_stride + key] : 0.f;
-        a.out[h * a.out_stride + key] = old + w[i];
-      }
+      const float v = __shfl_sync(0xffffffffu, w[i], 4 * (lane & 7));   // key 8 i + lane % 8
+      if ((lane >> 3) == i) mine = v;
     }
+    const int key = page * kBlockTokens + lane;
+    if (key < kv_end) a.out[h * a.out_stride + key] = fmaf(a.decay, old, mine);
+  };
+  auto load_prev = [&](int page) -> float {
+    const int key = page * kBlockTokens + lane;
+    return a.prev && page < pg1 && key < kv_end ? a.prev[h * a.prev_stride + key] : 0.f;
   };
 
+  float old_next = load_prev(first);
   bool ok = true;
   int st = 0, next = first + issued * W;
   uint32_t phase = 0;
@@ -889,24 +1006,26 @@ __global__ __launch_bounds__(Kv8Weights<D>::kThreads, D == 64 ? 2 : 1) void kv8_
     const uint8_t* sec = ring + st * L::kStageBytes;
     const float kc = reinterpret_cast<const float*>(sec)[0] * kCodeUnit<E4M3> * a.qk_scale;
     const bool open = page_open(page, a.ctx_len, a.m, a.window);
+    const float old = old_next;
+    old_next = load_prev(page + W);
+    uint32_t f[2][4 * NE][4];
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt) {
       const uint4* kc4 = reinterpret_cast<const uint4*>(sec + S::kOffK) + (mt * 2 * NE) * 32 + lane;
-      uint32_t f[4 * NE][4];
 #pragma unroll
       for (int e = 0; e < NE; ++e) {
         const uint4 ra = kc4[e * 32], rb = kc4[(NE + e) * 32];
         const uint32_t wa[4] = {ra.x, ra.y, ra.z, ra.w}, wb[4] = {rb.x, rb.y, rb.z, rb.w};
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-          f[4 * e + u][0] = decode_pair<E4M3, false>(wa[u]);
-          f[4 * e + u][1] = decode_pair<E4M3, false>(wb[u]);
-          f[4 * e + u][2] = decode_pair<E4M3, true>(wa[u]);
-          f[4 * e + u][3] = decode_pair<E4M3, true>(wb[u]);
+          f[mt][4 * e + u][0] = decode_pair<E4M3, false>(wa[u]);
+          f[mt][4 * e + u][1] = decode_pair<E4M3, false>(wb[u]);
+          f[mt][4 * e + u][2] = decode_pair<E4M3, true>(wa[u]);
+          f[mt][4 * e + u][3] = decode_pair<E4M3, true>(wb[u]);
         }
       }
-      rows16(f, page * kBlockTokens + 16 * mt, open, kc);
     }
+    rows32(f, page, open, kc, old);
     __syncwarp();
     if (next < pg1 && next < sealed_pages) {
       if (lane == 0) issue(next, st);
@@ -931,25 +1050,22 @@ __global__ __launch_bounds__(Kv8Weights<D>::kThreads, D == 64 ? 2 : 1) void kv8_
   int page = first;
   if (page < sealed_pages) page += (sealed_pages - page + W - 1) / W * W;
   for (; page < pg1; page += W) {
-#pragma unroll 1
-    for (int mt = 0; mt < 2; ++mt) {
-      const int key0 = page * kBlockTokens + 16 * mt;
-      if (key0 >= kv_end) break;
-      uint32_t f[4 * NE][4];
+    uint32_t f[2][4 * NE][4];
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
       for (int e = 0; e < NE; ++e) {
         uint2 kA[4], kB[4];
-        tail_k_frag<D>(tail, key0, e, g, c, kA, kB);
+        tail_k_frag<D>(tail, page * kBlockTokens + 16 * mt, e, g, c, kA, kB);
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-          f[4 * e + u][0] = kA[u].x;
-          f[4 * e + u][1] = kB[u].x;
-          f[4 * e + u][2] = kA[u].y;
-          f[4 * e + u][3] = kB[u].y;
+          f[mt][4 * e + u][0] = kA[u].x;
+          f[mt][4 * e + u][1] = kB[u].x;
+          f[mt][4 * e + u][2] = kA[u].y;
+          f[mt][4 * e + u][3] = kB[u].y;
         }
       }
-      rows16(f, key0, false, a.qk_scale);
-    }
+    rows32(f, page, false, a.qk_scale, load_prev(page));
   }
 }
 

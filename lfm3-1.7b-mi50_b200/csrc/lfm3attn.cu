@@ -62,9 +62,12 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) ==
 cudaStream_t as_stream(void* s) { return reinterpret_cast<cudaStream_t>(s); }
 
 int current_sm_count() {
+  static std::atomic<int> known[64];   // per device, asked once
   int dev = 0, n = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return 148;
+  if (dev >= 0 && dev < 64 && (n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
   if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) return 148;
+  if (dev >= 0 && dev < 64) known[dev].store(n, std::memory_order_relaxed);
   return n;
 }
 
@@ -1272,6 +1275,7 @@ int lfm3a_kv8_append(const lfm3a_kv8_view* kv, const void* k, const void* v, int
   a.a.n = n;
   a.tail = static_cast<__half*>(kv->tail);
   a.seal_page_end = seal_end;
+  a.vec = token_stride % 8 == 0 && aligned16(k) && aligned16(v);
   const cudaStream_t st = as_stream(stream);
   auto run = [&](int p0, int p1) -> int {
     if (p1 <= p0) return LFM3A_OK;
@@ -1302,7 +1306,7 @@ int lfm3a_kv8_read(const lfm3a_kv8_view* kv, int pos0, int n, int sealed, void* 
                 pos0, n, sealed};
   const dim3 grid((pos0 + n - 1) / kBlockTokens - pos0 / kBlockTokens + 1, L.kv_heads);
   with_format(L, [&](auto d, auto f) {
-    launch_pdl(kv8_read_kernel<decltype(d)::value, decltype(f)::value>, grid, 256, 0, as_stream(stream), a);
+    launch_pdl(kv8_read_kernel<decltype(d)::value, decltype(f)::value>, grid, 128, 0, as_stream(stream), a);
     return 0;
   });
   return check_launch("kv8_read_kernel");
@@ -1459,7 +1463,7 @@ int lfm3a_kv8_prefill(const lfm3a_kv8_view* kv, const void* q, int64_t q_stride,
   e.len = len;
   const cudaStream_t st = as_stream(stream);
   with_format(L, [&](auto d, auto f) {
-    launch_pdl(kv8_expand_kernel<decltype(d)::value, decltype(f)::value>, dim3(staged, H), 256, 0, st, e);
+    launch_pdl(kv8_expand_kernel<decltype(d)::value, decltype(f)::value>, dim3(staged, H), 128, 0, st, e);
     return 0;
   });
   rc = check_launch("kv8_expand_kernel");
@@ -1522,8 +1526,8 @@ int lfm3a_kv8_weights(const lfm3a_kv8_view* kv, const void* q, int64_t q_stride,
   a.pages = (len + kBlockTokens - 1) / kBlockTokens;
   a.decay = decay;
   a.qk_scale = (1.f / sqrtf((float)D)) * kLog2e;
-  const int target = (D == 64 ? 2 : 1) * current_sm_count();
-  a.splits = std::max(1, std::min(target / H, (a.pages + 7) / 8));
+  // Two blocks per SM (up to 128 rows; more rows' operands leave room for one), a page for each of a block's 8 warps.
+  a.splits = std::max(1, std::min(2 * current_sm_count() / H, (a.pages + 7) / 8));
   const int ntiles = (m * group + 7) / 8;
   const cudaStream_t st = as_stream(stream);
   static std::atomic<bool> done[4][64];
@@ -1546,8 +1550,13 @@ int lfm3a_evict_select(const float* weights, int64_t stride, int kv_heads, int l
   if (stride < len || (weights_out && out_stride < budget)) return fail(LFM3A_EINVAL, "a row of weights is too short");
   if (sink < 0 || recent < 0 || budget < 1 || budget > len || (int64_t)sink + recent > budget)
     return fail(LFM3A_EINVAL, "need sink + recent <= budget <= len");
-  EvictArgs a{weights, keep, weights_out, stride, out_stride, len, sink, recent, budget};
-  launch_pdl(evict_select_kernel, dim3(kEvictCluster, kv_heads), kEvictThreads, 0, as_stream(stream), a);
+  const int share = (len - sink - recent + kEvictCluster - 1) / kEvictCluster;
+  EvictArgs a{weights, keep, weights_out, stride, out_stride, len, sink, recent, budget, share <= kEvictCache};
+  static std::atomic<bool> done[64];
+  const int rc = ensure_smem(evict_select_kernel, kEvictCache * (int)sizeof(uint32_t), done);
+  if (rc != LFM3A_OK) return rc;
+  launch_pdl(evict_select_kernel, dim3(kEvictCluster, kv_heads), kEvictThreads, a.cached ? share * sizeof(uint32_t) : 0,
+             as_stream(stream), a);
   return check_launch("evict_select_kernel");
 }
 

@@ -159,6 +159,8 @@ SIGNATURES = {
 }
 
 _lib = None
+_torch = None   # imported on first use
+_raw_stream = None
 
 
 def lib() -> ctypes.CDLL:
@@ -190,9 +192,18 @@ def _ptr(t) -> int | None:
 
 def _stream(stream) -> int | None:
     if stream is None:
-        import torch
+        global _torch, _raw_stream
+        if _torch is None:
+            import torch
 
-        return torch.cuda.current_stream().cuda_stream
+            _torch = torch
+            # the raw handle of the current stream: 0.1 us where the stream object takes 3
+            raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+            if raw is not None:
+                _raw_stream = raw
+        if _raw_stream is not None:
+            return _raw_stream(_torch.cuda.current_device())
+        return _torch.cuda.current_stream().cuda_stream
     if isinstance(stream, int):
         return stream
     return stream.cuda_stream
@@ -502,6 +513,11 @@ class LayerCache8:
         self.view = Kv8View(KvView(self.pool.data_ptr(), self.table.data_ptr(), self.pool_blocks, self.layout),
                             self.tail.data_ptr())
         self._view = ctypes.byref(self.view)
+        # a decoded token's calls take a few us on the GPU: what they look up per call is kept here
+        handle = lib()
+        self._append, self._read, self._attention = handle.lfm3a_kv8_append, handle.lfm3a_kv8_read, handle.lfm3a_kv8_attention
+        self._weights, self._compact = handle.lfm3a_kv8_weights, handle.lfm3a_kv8_compact
+        self._new, self._like, self._f16, self._f32 = torch.empty, torch.empty_like, torch.float16, torch.float32
 
     def workspace(self, tokens: int, q_heads: int):
         """A device workspace for verify (up to 32 tokens) and prefill calls of this many tokens at any length."""
@@ -529,8 +545,8 @@ class LayerCache8:
         if pos0 > self.length:
             raise LFM3AError(EINVAL, "append would leave a gap")
         seal_to = pos0 if draft else pos0 + n
-        _check(lib().lfm3a_kv8_append(self._view, _ptr(k), _ptr(v), token_stride, pos0, n, self.sealed, seal_to,
-                                      _ptr(rope), _ptr(k_norm), _stream(stream)))
+        _check(self._append(self._view, _ptr(k), _ptr(v), token_stride, pos0, n, self.sealed, seal_to, _ptr(rope),
+                            _ptr(k_norm), _stream(stream)))
         self.sealed = seal_to // BLOCK_TOKENS * BLOCK_TOKENS
         self.length = pos0 + n
 
@@ -542,39 +558,36 @@ class LayerCache8:
 
     def read(self, pos0: int, n: int, stream=None):
         """(K, V) fp16 [n][kv_heads][head_dim]: the values the cached tokens pos0.. stand for."""
-        import torch
-
         if pos0 < 0 or n < 0 or pos0 + n > self.length:
             raise LFM3AError(EINVAL, "read past the cached tokens")
-        k, v = (torch.empty((n, self.kv_heads, self.head_dim), dtype=torch.float16, device=self.pool.device)
-                for _ in range(2))
-        _check(lib().lfm3a_kv8_read(self._view, pos0, n, self.sealed, _ptr(k), _ptr(v), _stream(stream)))
+        k = self._new((n, self.kv_heads, self.head_dim), dtype=self._f16, device=self.pool.device)
+        v = self._like(k)
+        _check(self._read(self._view, pos0, n, self.sealed, k.data_ptr(), v.data_ptr(), _stream(stream)))
         return k, v
 
     def _check_q(self, q, ctx_len: int) -> tuple[int, int, int]:
         m, qh, d = q.shape
-        if d != self.head_dim or q.stride(2) != 1 or (qh > 1 and q.stride(1) != d):
+        st, sh, sd = q.stride()
+        if d != self.head_dim or sd != 1 or (qh > 1 and sh != d):
             raise LFM3AError(EINVAL, "q must be [tokens][q_heads][head_dim] with contiguous rows")
         if ctx_len < 0 or ctx_len + m > self.length:
             raise LFM3AError(EINVAL, "the queries' tokens must be appended first")
-        return m, qh, q.stride(0) if m > 1 else qh * d
+        return m, qh, st if m > 1 else qh * d
 
     def verify(self, q, ctx_len: int, window: int = 0, gate=None, out=None, lse=None, workspace=None, splits: int = 0,
                stream=None):
         """Attention of q ([m][q_heads][head_dim] fp16, row-strided) at ctx_len.., m <= 32; the tokens' K/V appended.
         lse: fp32 [m][q_heads] to fill with each row's log-sum-exp. Returns fp16 [m][q_heads][head_dim]."""
-        import torch
-
         m, qh, stride = self._check_q(q, ctx_len)
         if out is None:
-            out = torch.empty((m, qh, self.head_dim), dtype=torch.float16, device=q.device)
+            out = self._like(q) if q.is_contiguous() else self._new(q.shape, dtype=self._f16, device=q.device)
         if workspace is None:
             s = splits if splits > 0 else self.splits(qh, ctx_len, m, window)
-            workspace = torch.empty(lib().lfm3a_verify_workspace_bytes(m, qh, self.head_dim, s), dtype=torch.uint8,
-                                    device=q.device)
-        _check(lib().lfm3a_kv8_attention(self._view, _ptr(q), stride, m, qh, ctx_len, self.sealed_below(ctx_len + m),
-                                         window, _ptr(gate), _ptr(out), _ptr(lse), _ptr(workspace), workspace.numel(),
-                                         splits, _stream(stream)))
+            workspace = self._new(lib().lfm3a_verify_workspace_bytes(m, qh, self.head_dim, s) // 4, dtype=self._f32,
+                                  device=q.device)
+        _check(self._attention(self._view, q.data_ptr(), stride, m, qh, ctx_len, self.sealed_below(ctx_len + m), window,
+                               _ptr(gate), out.data_ptr(), _ptr(lse), workspace.data_ptr(), workspace.nbytes, splits,
+                               _stream(stream)))
         return out
 
     def sealed_below(self, length: int) -> int:
@@ -602,20 +615,18 @@ class LayerCache8:
     def key_weights(self, q, lse, ctx_len: int, window: int = 0, prev=None, decay: float = 1.0, out=None, stream=None):
         """fp32 [kv_heads][ctx_len + m]: decay * prev plus the attention weight each key got from the m tokens of q,
         summed over the query heads of its kv head. lse: of verify for the same q."""
-        import torch
-
         m, qh, stride = self._check_q(q, ctx_len)
-        if lse.dtype != torch.float32 or tuple(lse.shape) != (m, qh) or not lse.is_contiguous():
+        if lse.dtype != self._f32 or tuple(lse.shape) != (m, qh) or not lse.is_contiguous():
             raise LFM3AError(EINVAL, "lse must be fp32 [m][q_heads]")
         n = ctx_len + m
         if out is None:
-            out = torch.empty((self.kv_heads, n), dtype=torch.float32, device=q.device)
+            out = self._new((self.kv_heads, n), dtype=self._f32, device=q.device)
         for t in (out, prev):
-            if t is not None and (t.dtype != torch.float32 or t.shape[0] != self.kv_heads or t.stride(1) != 1):
+            if t is not None and (t.dtype != self._f32 or t.shape[0] != self.kv_heads or t.stride(1) != 1):
                 raise LFM3AError(EINVAL, "weights must be fp32 [kv_heads][>= ctx_len + m]")
-        _check(lib().lfm3a_kv8_weights(self._view, _ptr(q), stride, m, qh, ctx_len, self.sealed_below(n), window,
-                                       _ptr(lse), _ptr(prev), 0 if prev is None else prev.stride(0), decay, _ptr(out),
-                                       out.stride(0), _stream(stream)))
+        _check(self._weights(self._view, q.data_ptr(), stride, m, qh, ctx_len, self.sealed_below(n), window,
+                             lse.data_ptr(), _ptr(prev), 0 if prev is None else prev.stride(0), decay, out.data_ptr(),
+                             out.stride(0), _stream(stream)))
         return out
 
     def evict(self, weights, budget: int, sink: int, recent: int, dst: "LayerCache8", stream=None):
@@ -625,8 +636,7 @@ class LayerCache8:
         if dst is self or budget > dst.capacity:
             raise LFM3AError(EINVAL, "eviction needs another cache with room for the budget")
         keep, kept = evict_select(weights, self.length, budget, sink, recent, stream=stream)
-        _check(lib().lfm3a_kv8_compact(self._view, self.length, self.sealed, _ptr(keep), budget, dst._view,
-                                       _stream(stream)))
+        _check(self._compact(self._view, self.length, self.sealed, keep.data_ptr(), budget, dst._view, _stream(stream)))
         dst.length, dst.sealed = budget, budget // BLOCK_TOKENS * BLOCK_TOKENS
         return keep, kept
 
