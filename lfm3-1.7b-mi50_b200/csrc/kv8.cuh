@@ -53,23 +53,58 @@ __host__ __device__ __forceinline__ TailView tail_of(__half* tail, int kv_heads,
 // fp16 values of the cache are finite: NaN becomes 0, an infinity the largest finite value of its sign.
 __device__ __forceinline__ float finite_f16(float x) { return x != x ? 0.f : fminf(fmaxf(x, -65504.f), 65504.f); }
 
-// The 8-bit code of the fp32 quotient x / scale, to nearest even (inv: the rounded reciprocal of scale, |x| at most 127
-// or 448 scales). x * inv is within 2^-22 of the quotient, relatively, so it decides the code unless a rounding boundary
-// lies that near; then the division itself does. (Dividing every value took half of the append kernel's time.)
+// Four words of 8-bit codes, byte b of word k being the code of the fp32 quotient v[k][b] / scale, to nearest even (inv:
+// the rounded reciprocal of scale; no value is beyond 127 or 448 scales). v * inv is within 2^-22 of the quotient,
+// relatively, so it decides a code unless a rounding boundary lies that near; if one does for any of the 16, the
+// divisions themselves decide all of them. (Dividing every value took half of the append kernel's time, a branch per
+// value another quarter.)
 template <bool E4M3>
-__device__ __forceinline__ uint32_t encode8(float x, float scale, float inv) {
+__device__ __forceinline__ void encode16(const float (&v)[4][4], float scale, float inv, uint32_t (&w)[4]) {
   if (E4M3) {   // saturating at 448
-    const float y = x * inv;
-    uint16_t r;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(y * (1.f + 0x1p-21f)), "f"(y * (1.f - 0x1p-21f)));
-    if ((r >> 8) != (r & 0xffu))
-      asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(0.f), "f"(__fdiv_rn(x, scale)));
-    return (uint32_t)r & 0xffu;
+    auto pair = [](float lo, float hi) {
+      uint16_t r;
+      asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+      return (uint32_t)r;
+    };
+    uint32_t doubt = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      uint32_t r[2];
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const float y0 = v[k][2 * b] * inv, y1 = v[k][2 * b + 1] * inv;
+        r[b] = pair(y0 * (1.f + 0x1p-21f), y1 * (1.f + 0x1p-21f));
+        doubt |= r[b] ^ pair(y0 * (1.f - 0x1p-21f), y1 * (1.f - 0x1p-21f));
+      }
+      w[k] = __byte_perm(r[0], r[1], 0x5410);
+    }
+    if (doubt) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        w[k] = __byte_perm(pair(__fdiv_rn(v[k][0], scale), __fdiv_rn(v[k][1], scale)),
+                           pair(__fdiv_rn(v[k][2], scale), __fdiv_rn(v[k][3], scale)), 0x5410);
+    }
+    return;
   }
   constexpr float kMagic = 12582912.f;   // 1.5 * 2^23: adding it rounds to an integer, whose low byte is the code
-  float t = fmaf(x, inv, kMagic);
-  if (fabsf(fmaf(x, inv, kMagic - t)) > 0.4999f) t = __fdiv_rn(x, scale) + kMagic;
-  return __float_as_uint(t) & 0xffu;
+  float t[4][4], worst = 0.f;
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      t[k][b] = fmaf(v[k][b], inv, kMagic);
+      worst = fmaxf(worst, fabsf(fmaf(v[k][b], inv, kMagic - t[k][b])));
+    }
+  if (worst > 0.49998f) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int b = 0; b < 4; ++b) t[k][b] = __fdiv_rn(v[k][b], scale) + kMagic;
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    w[k] = __byte_perm(__byte_perm(__float_as_uint(t[k][0]), __float_as_uint(t[k][1]), 0x0040),
+                       __byte_perm(__float_as_uint(t[k][2]), __float_as_uint(t[k][3]), 0x0040), 0x5410);
 }
 
 // Bytes 0, 1 (LO) or 2, 3 of a word of codes as an fp16 pair. int8: 0x64NN is 1024 + NN with NN = v ^ 0x80, minus
@@ -103,17 +138,15 @@ __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
 }
 
 // ---------------------------------------------------------------- append and sealing
-// Seals one page and kv head from fp32 rows in shared memory (x [2][32][kSealRow]: K, then V), by 256 threads, each with
-// the largest magnitude of the K and V values it put there. codes: 32 D bytes of shared memory. A thread makes 16 codes
-// at a time: a whole 16-byte chunk of K, which goes out as it is, or 4 dims x 4 keys of V, four words of four chunks,
-// which are put in order in shared memory first.
-constexpr int kSealThreads = 256;
+// A page and kv head is sealed by 2 D threads: the first half of them makes K's codes, the other V's, 16 at a time, two
+// times each. Each gives the largest magnitude of the K and of the V values it has seen and gets the scale of its half
+// and the rounded reciprocal; the header (both scales, zeros) is written. The barrier inside also publishes shared memory
+// written before.
 template <int D>
-constexpr int kSealRow = D + 4;   // floats; 16-byte aligned rows
+constexpr int kSealThreads = 2 * D;
 template <int D, bool E4M3>
-__device__ __forceinline__ void seal_page(const float* x, float kmax, float vmax, float* red, uint8_t* codes, char* sec) {
-  using S = Q8Section<D>;
-  constexpr int RS = kSealRow<D>;
+__device__ __forceinline__ float2 seal_scale(float kmax, float vmax, float* red, char* sec) {
+  constexpr int W = kSealThreads<D> / 32;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 #pragma unroll
   for (int o = 16; o >= 1; o >>= 1) {
@@ -122,77 +155,107 @@ __device__ __forceinline__ void seal_page(const float* x, float kmax, float vmax
   }
   if (lane == 0) {
     red[warp] = kmax;
-    red[8 + warp] = vmax;
-  }
-  __syncthreads();   // also publishes x
-  float scale[2], inv[2];
-#pragma unroll
-  for (int s = 0; s < 2; ++s) {
-    float amax = red[8 * s];
-#pragma unroll
-    for (int w = 1; w < 8; ++w) amax = fmaxf(amax, red[8 * s + w]);
-    scale[s] = amax > 0.f ? __fdiv_rn(amax, E4M3 ? 448.f : 127.f) : 1.f;
-    inv[s] = __fdiv_rn(1.f, scale[s]);
-  }
-  if (tid < 8) reinterpret_cast<float*>(sec)[tid] = tid < 2 ? scale[tid] : 0.f;
-  uint4* K = reinterpret_cast<uint4*>(sec + S::kOffK);
-  const float* v = x + 32 * RS;
-  for (int i = tid; i < 4 * D; i += kSealThreads) {
-    if (i < 2 * D) {   // 16 dims of one key
-      const int l = i & 31, a = i >> 5;
-      const int key = (a / (D / 64)) * 8 + (l >> 2), dim0 = (a % (D / 64)) * 64 + (l & 3) * 16;
-      uint32_t w[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float4 f = *reinterpret_cast<const float4*>(x + key * RS + dim0 + 4 * k);
-        w[k] = encode8<E4M3>(f.x, scale[0], inv[0]) | encode8<E4M3>(f.y, scale[0], inv[0]) << 8 |
-               encode8<E4M3>(f.z, scale[0], inv[0]) << 16 | encode8<E4M3>(f.w, scale[0], inv[0]) << 24;
-      }
-      K[i] = make_uint4(w[0], w[1], w[2], w[3]);
-    } else {           // dims dim0 .. + 3 of keys key0, + 1, + 8, + 9
-      const int k = i - 2 * D, c = k & 3, wi = (k >> 2) & 3, gh = (k >> 4) & 1, dtp = (k >> 5) % (D / 32), mt = (k >> 5) / (D / 32);
-      const int key0 = 16 * mt + 2 * c, dim0 = 32 * dtp + 16 * (wi >> 1) + 8 * (wi & 1) + 4 * gh;
-      uint32_t w[4] = {0, 0, 0, 0};
-#pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        const float4 f = *reinterpret_cast<const float4*>(v + (key0 + (b & 1) + 8 * (b >> 1)) * RS + dim0);
-        w[0] |= encode8<E4M3>(f.x, scale[1], inv[1]) << (8 * b);
-        w[1] |= encode8<E4M3>(f.y, scale[1], inv[1]) << (8 * b);
-        w[2] |= encode8<E4M3>(f.z, scale[1], inv[1]) << (8 * b);
-        w[3] |= encode8<E4M3>(f.w, scale[1], inv[1]) << (8 * b);
-      }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) *reinterpret_cast<uint32_t*>(codes + S::v_index(key0, dim0 + e)) = w[e];
-    }
+    red[W + warp] = vmax;
   }
   __syncthreads();
-  uint4* V = reinterpret_cast<uint4*>(sec + S::kOffV);
-  for (int i = tid; i < 2 * D; i += kSealThreads) V[i] = reinterpret_cast<const uint4*>(codes)[i];
+  const bool is_v = tid >= D;
+  const float4* r = reinterpret_cast<const float4*>(red + (is_v ? W : 0));
+  float amax = 0.f;
+#pragma unroll
+  for (int i = 0; i < W / 4; ++i) amax = fmaxf(amax, fmaxf(fmaxf(r[i].x, r[i].y), fmaxf(r[i].z, r[i].w)));
+  const float scale = amax > 0.f ? __fdiv_rn(amax, E4M3 ? 448.f : 127.f) : 1.f;
+  if (lane < 4 && (warp == 0 || warp == W / 2)) reinterpret_cast<float*>(sec)[2 * lane + is_v] = lane ? 0.f : scale;
+  return make_float2(scale, __fdiv_rn(1.f, scale));
 }
 
-__device__ __forceinline__ void unpack_row8(uint4 v, float (&f)[8]) {
+template <int D>
+constexpr int kSealRow = D + 8;   // halves of a staged row; 16-byte aligned rows
+__device__ __forceinline__ void unpack4(uint2 h, float (&f)[4]) {
+  const float2 a = unpack_half2(h.x), b = unpack_half2(h.y);
+  f[0] = a.x;
+  f[1] = a.y;
+  f[2] = b.x;
+  f[3] = b.y;
+}
+// Seals fp16 rows staged in shared memory (x [2][32][kSealRow]: K, then V). A thread makes a whole 16-byte chunk of K at a
+// time, or 4 dims x 4 keys of V: four words, of which 16 lanes' fill 64 bytes.
+template <int D, bool E4M3>
+__device__ __forceinline__ void seal_page(const __half* x, float kmax, float vmax, float* red, char* sec) {
+  using S = Q8Section<D>;
+  constexpr int RS = kSealRow<D>;
+  const int tid = threadIdx.x;
+  const float2 sc = seal_scale<D, E4M3>(kmax, vmax, red, sec);
+  uint32_t w[4];
+  float v[4][4];
+  if (tid < D) {
+    uint4* K = reinterpret_cast<uint4*>(sec + S::kOffK);
+#pragma unroll
+    for (int i = tid; i < 2 * D; i += D) {   // 16 dims of one key
+      const int l = i & 31, a = i >> 5;
+      const int key = (a / (D / 64)) * 8 + (l >> 2), dim0 = (a % (D / 64)) * 64 + (l & 3) * 16;
+      const uint4* src = reinterpret_cast<const uint4*>(x + key * RS + dim0);
+      const uint4 a0 = src[0], a1 = src[1];
+      unpack4(make_uint2(a0.x, a0.y), v[0]);
+      unpack4(make_uint2(a0.z, a0.w), v[1]);
+      unpack4(make_uint2(a1.x, a1.y), v[2]);
+      unpack4(make_uint2(a1.z, a1.w), v[3]);
+      encode16<E4M3>(v, sc.x, sc.y, w);
+      K[i] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  } else {
+    uint8_t* V = reinterpret_cast<uint8_t*>(sec + S::kOffV);
+#pragma unroll
+    for (int i = tid - D; i < 2 * D; i += D) {   // dims dim0 .. + 3 of 4 keys
+      const int c = i & 3, wi = (i >> 2) & 3, gh = (i >> 4) & 1, dtp = (i >> 5) % (D / 32), mt = (i >> 5) / (D / 32);
+      const int key0 = 16 * mt + 2 * c, dim0 = 32 * dtp + 16 * (wi >> 1) + 8 * (wi & 1) + 4 * gh;
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        float f[4];
+        unpack4(*reinterpret_cast<const uint2*>(x + (32 + key0 + (b & 1) + 8 * (b >> 1)) * RS + dim0), f);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e][b] = f[e];
+      }
+      encode16<E4M3>(v, sc.x, sc.y, w);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) *reinterpret_cast<uint32_t*>(V + S::v_index(key0, dim0 + e)) = w[e];
+    }
+  }
+}
+
+// 8 halves at p (16-byte aligned when vec).
+__device__ __forceinline__ uint4 load_row8(const __half* p, bool vec) {
+  if (vec) return *reinterpret_cast<const uint4*>(p);
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __half2 h = __halves2half2(p[2 * i], p[2 * i + 1]);
+    w[i] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// Largest magnitude of 8 halves, NaN if one is.
+__device__ __forceinline__ __half2 max_abs8(uint4 v, __half2 m) {
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float2 p = unpack_half2(w[i]);
-    f[2 * i] = finite_f16(p.x);
-    f[2 * i + 1] = finite_f16(p.y);
+    const uint32_t a = w[i] & 0x7fff7fffu;
+    m = __hmax2_nan(m, *reinterpret_cast<const __half2*>(&a));
   }
+  return m;
 }
-// 8 halves at p (16-byte aligned when vec) as finite floats into dst (16-byte aligned); returns their largest magnitude.
-__device__ __forceinline__ float stage_row8(const __half* p, bool vec, float* dst) {
-  float f[8];
-  if (vec) {
-    unpack_row8(*reinterpret_cast<const uint4*>(p), f);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = finite_f16(__half2float(p[i]));
-  }
-  *reinterpret_cast<float4*>(dst) = make_float4(f[0], f[1], f[2], f[3]);
-  *reinterpret_cast<float4*>(dst + 4) = make_float4(f[4], f[5], f[6], f[7]);
+__device__ __forceinline__ float max_of(__half2 m) {
+  const __half h = __hmax_nan(__low2half(m), __high2half(m));
+  return __half2float(h);
+}
+// Makes 8 halves finite in place; returns their largest magnitude.
+__device__ __forceinline__ float make_finite8(__half* p) {
   float m = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(f[i]));
+  for (int i = 0; i < 8; ++i) {
+    const float f = finite_f16(__half2float(p[i]));
+    p[i] = __float2half_rn(f);
+    m = fmaxf(m, fabsf(f));
+  }
   return m;
 }
 
@@ -208,11 +271,10 @@ struct Kv8AppendArgs {
 // a load; K through the fp16 k-norm and RoPE that lfm3a_kv_append applies). Bound by memory for prompt chunks, by the
 // latency of one round of loads for drafts.
 template <int D, bool E4M3>
-__global__ __launch_bounds__(kSealThreads) void kv8_append_kernel(Kv8AppendArgs args) {
+__global__ __launch_bounds__(kSealThreads<D>) void kv8_append_kernel(Kv8AppendArgs args) {
   constexpr int J = D / 64, HALF = D / 2, RS = kSealRow<D>, R8 = D / 8;
-  __shared__ __align__(16) float x[2 * 32 * RS];
-  __shared__ __align__(16) uint8_t codes[32 * D];
-  __shared__ float red[16];
+  __shared__ __align__(16) __half x[2 * 32 * RS];
+  __shared__ __align__(16) float red[16];
   pdl_wait();
   pdl_trigger();
   const AppendArgs& a = args.a;
@@ -223,58 +285,90 @@ __global__ __launch_bounds__(kSealThreads) void kv8_append_kernel(Kv8AppendArgs 
   if (!sealing && lo >= end) return;
   const TailView tail = tail_of(args.tail, a.g.kv_heads, h, D);
   float kmax = 0.f, vmax = 0.f;
+  {
+    constexpr int U = kBlockTokens * R8 / kSealThreads<D>;   // 16-byte pieces of K and of V per thread
+    uint4 kr[U], vr[U];
+    const uint4 zero = make_uint4(0, 0, 0, 0);
 #pragma unroll
-  for (int i = tid; i < kBlockTokens * R8; i += kSealThreads) {
-    const int r = i / R8, d = (i % R8) * 8, t = t0 + r;
-    if (t < lo || t >= end) continue;
-    const int64_t at = (int64_t)(t - a.pos0) * a.stride + h * D + d;
-    if (plain) kmax = fmaxf(kmax, stage_row8(a.k + at, vec, x + r * RS + d));
-    vmax = fmaxf(vmax, stage_row8(a.v + at, vec, x + (32 + r) * RS + d));
+    for (int u = 0; u < U; ++u) {
+      const int i = tid + u * kSealThreads<D>, t = t0 + i / R8;
+      const bool live = t >= lo && t < end;
+      const int64_t at = (int64_t)(t - a.pos0) * a.stride + h * D + (i % R8) * 8;
+      kr[u] = live && plain ? load_row8(a.k + at, vec) : zero;
+      vr[u] = live ? load_row8(a.v + at, vec) : zero;
+    }
+    __half2 km = __float2half2_rn(0.f), vm = km;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = tid + u * kSealThreads<D>, r = i / R8, d = (i % R8) * 8;
+      if (t0 + r >= lo && t0 + r < end) {
+        if (plain) *reinterpret_cast<uint4*>(x + r * RS + d) = kr[u];
+        *reinterpret_cast<uint4*>(x + (32 + r) * RS + d) = vr[u];
+      }
+      km = max_abs8(kr[u], km);
+      vm = max_abs8(vr[u], vm);
+    }
+    kmax = max_of(km);
+    vmax = max_of(vm);
+    if (!(kmax <= 65504.f) || !(vmax <= 65504.f)) {   // an infinity or NaN among this thread's values
+      kmax = vmax = 0.f;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int i = tid + u * kSealThreads<D>, r = i / R8, d = (i % R8) * 8;
+        if (t0 + r < lo || t0 + r >= end) continue;
+        if (plain) kmax = fmaxf(kmax, make_finite8(x + r * RS + d));
+        vmax = fmaxf(vmax, make_finite8(x + (32 + r) * RS + d));
+      }
+    }
   }
   if (!plain) {
 #pragma unroll 4
-    for (int t = lo + warp; t < end; t += 8) {
+    for (int t = lo + warp; t < end; t += kSealThreads<D> / 32) {
       float ra[J], rb[J];
       norm_rope_pairs<D>(a, a.k + (int64_t)(t - a.pos0) * a.stride + h * D, t, lane, ra, rb);
-      float* row = x + (t - t0) * RS;
+      __half* row = x + (t - t0) * RS;
 #pragma unroll
       for (int j = 0; j < J; ++j) {
         const float k0 = finite_f16(ra[j]), k1 = finite_f16(rb[j]);
-        row[lane + 32 * j] = k0;
-        row[lane + 32 * j + HALF] = k1;
+        row[lane + 32 * j] = __float2half_rn(k0);
+        row[lane + 32 * j + HALF] = __float2half_rn(k1);
         kmax = fmaxf(kmax, fmaxf(fabsf(k0), fabsf(k1)));
       }
     }
   }
   if (!sealing) {
     __syncthreads();
-    for (int i = tid; i < (end - lo) * D; i += kSealThreads) {
+    for (int i = tid; i < (end - lo) * D; i += kSealThreads<D>) {
       const int t = lo + i / D, d = i % D, slot = t % kTailTokens;
-      tail.k[(int64_t)slot * D + d] = __float2half_rn(x[(t - t0) * RS + d]);
-      tail.v[(int64_t)d * kTailTokens + slot] = __float2half_rn(x[(32 + t - t0) * RS + d]);
+      tail.k[(int64_t)slot * D + d] = x[(t - t0) * RS + d];
+      tail.v[(int64_t)d * kTailTokens + slot] = x[(32 + t - t0) * RS + d];
     }
     return;
   }
-  if (lo > t0) {   // tokens that wait in the tail
+  if (lo > t0) {   // tokens that wait in the tail (finite already)
     const int old = min(lo, t0 + kBlockTokens) - t0, slot0 = t0 % kTailTokens;
-    for (int i = tid; i < old * R8; i += kSealThreads) {
+    __half2 km = __float2half2_rn(0.f);
+    for (int i = tid; i < old * R8; i += kSealThreads<D>) {
       const int r = i / R8, d = (i % R8) * 8;
-      kmax = fmaxf(kmax, stage_row8(tail.k + (int64_t)(slot0 + r) * D + d, true, x + r * RS + d));
+      const uint4 v = *reinterpret_cast<const uint4*>(tail.k + (int64_t)(slot0 + r) * D + d);
+      *reinterpret_cast<uint4*>(x + r * RS + d) = v;
+      km = max_abs8(v, km);
     }
-    for (int i = tid; i < D * 4; i += kSealThreads) {   // 8 tokens of one dim
+    kmax = fmaxf(kmax, max_of(km));
+    for (int i = tid; i < D * 4; i += kSealThreads<D>) {   // 8 tokens of one dim
       const int d = i >> 2, r0 = (i & 3) * 8;
       if (r0 >= old) continue;
-      float f[8];
-      unpack_row8(*reinterpret_cast<const uint4*>(tail.v + (int64_t)d * kTailTokens + slot0 + r0), f);
+      const uint4 v = *reinterpret_cast<const uint4*>(tail.v + (int64_t)d * kTailTokens + slot0 + r0);
+      const __half* f = reinterpret_cast<const __half*>(&v);
 #pragma unroll
       for (int e = 0; e < 8; ++e)
         if (r0 + e < old) {
           x[(32 + r0 + e) * RS + d] = f[e];
-          vmax = fmaxf(vmax, fabsf(f[e]));
+          vmax = fmaxf(vmax, fabsf(__half2float(f[e])));
         }
     }
   }
-  seal_page<D, E4M3>(x, kmax, vmax, red, codes, a.g.pool + phys_block(a.g, page) * a.g.block_bytes + h * a.g.head_bytes);
+  seal_page<D, E4M3>(x, kmax, vmax, red, a.g.pool + phys_block(a.g, page) * a.g.block_bytes + h * a.g.head_bytes);
 }
 
 // ---------------------------------------------------------------- reading back
@@ -348,11 +442,25 @@ __global__ __launch_bounds__(128) void kv8_read_kernel(Kv8ReadArgs a) {
     }
   } else {
     const TailView tail = tail_of(a.tail, a.g.kv_heads, h, D);
-    for (int i = tid; i < (hi - lo) * D; i += 128) {
-      const int t = lo + i / D, d = i % D, slot = t % kTailTokens;
-      const int64_t at = (t - a.pos0) * row + d;
-      k_out[at] = tail.k[(int64_t)slot * D + d];
-      v_out[at] = tail.v[(int64_t)d * kTailTokens + slot];
+    const int slot0 = t0 % kTailTokens;
+    constexpr int U = D / 32;   // 8 values of K and of V per thread and round, all loads first
+    uint4 kr[U], vr[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = tid + 128 * u;
+      kr[u] = *reinterpret_cast<const uint4*>(tail.k + (int64_t)(slot0 + i / (D / 8)) * D + (i % (D / 8)) * 8);
+      vr[u] = *reinterpret_cast<const uint4*>(tail.v + (int64_t)(i % D) * kTailTokens + slot0 + (i / D) * 8);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = tid + 128 * u, t = t0 + i / (D / 8);
+      if (t >= lo && t < hi) *reinterpret_cast<uint4*>(k_out + (t - a.pos0) * row + (i % (D / 8)) * 8) = kr[u];
+      const __half* v = reinterpret_cast<const __half*>(&vr[u]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int tv = t0 + (i / D) * 8 + e;
+        if (tv >= lo && tv < hi) v_out[(tv - a.pos0) * row + i % D] = v[e];
+      }
     }
   }
 }

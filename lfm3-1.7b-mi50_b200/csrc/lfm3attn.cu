@@ -1281,7 +1281,8 @@ int lfm3a_kv8_append(const lfm3a_kv8_view* kv, const void* k, const void* v, int
     if (p1 <= p0) return LFM3A_OK;
     a.page0 = p0;
     rc = with_format(L, [&](auto d, auto f) {
-      launch_pdl(kv8_append_kernel<decltype(d)::value, decltype(f)::value>, dim3(p1 - p0, H), kSealThreads, 0, st, a);
+      launch_pdl(kv8_append_kernel<decltype(d)::value, decltype(f)::value>, dim3(p1 - p0, H),
+                 kSealThreads<decltype(d)::value>, 0, st, a);
       return LFM3A_OK;
     });
     return check_launch("kv8_append_kernel");
@@ -1550,12 +1551,15 @@ int lfm3a_evict_select(const float* weights, int64_t stride, int kv_heads, int l
   if (stride < len || (weights_out && out_stride < budget)) return fail(LFM3A_EINVAL, "a row of weights is too short");
   if (sink < 0 || recent < 0 || budget < 1 || budget > len || (int64_t)sink + recent > budget)
     return fail(LFM3A_EINVAL, "need sink + recent <= budget <= len");
-  const int share = (len - sink - recent + kEvictCluster - 1) / kEvictCluster;
+  const int n = len - sink - recent, blocks = n <= kEvictSingle ? 1 : 8, share = (n + blocks - 1) / blocks;
   EvictArgs a{weights, keep, weights_out, stride, out_stride, len, sink, recent, budget, share <= kEvictCache};
-  static std::atomic<bool> done[64];
-  const int rc = ensure_smem(evict_select_kernel, kEvictCache * (int)sizeof(uint32_t), done);
+  const size_t smem = a.cached ? share * sizeof(uint32_t) : 0;
+  constexpr int kMost = kEvictCache * (int)sizeof(uint32_t);
+  static std::atomic<bool> done[2][64];
+  const int rc = blocks == 1 ? ensure_smem(evict_select_kernel, kMost, done[0])
+                             : ensure_smem(evict_select_cluster_kernel, kMost, done[1]);
   if (rc != LFM3A_OK) return rc;
-  launch_pdl(evict_select_kernel, dim3(kEvictCluster, kv_heads), kEvictThreads, a.cached ? share * sizeof(uint32_t) : 0,
+  launch_pdl(blocks == 1 ? evict_select_kernel : evict_select_cluster_kernel, dim3(blocks, kv_heads), kEvictThreads, smem,
              as_stream(stream), a);
   return check_launch("evict_select_kernel");
 }
@@ -1576,7 +1580,8 @@ int lfm3a_kv8_compact(const lfm3a_kv8_view* src, int len, int sealed, const int3
                    keep, len, sealed, budget};
   const dim3 grid((budget + kBlockTokens - 1) / kBlockTokens, L.kv_heads);
   with_format(L, [&](auto d, auto f) {
-    launch_pdl(kv8_compact_kernel<decltype(d)::value, decltype(f)::value>, grid, kSealThreads, 0, as_stream(stream), a);
+    launch_pdl(kv8_compact_kernel<decltype(d)::value, decltype(f)::value>, grid, kSealThreads<decltype(d)::value>, 0,
+               as_stream(stream), a);
     return 0;
   });
   return check_launch("kv8_compact_kernel");
