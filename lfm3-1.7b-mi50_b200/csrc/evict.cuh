@@ -228,8 +228,8 @@ __global__ __launch_bounds__(kSealThreads<D>) void kv8_compact_kernel(Kv8Compact
   if (tid < 32 && sec[tid]) f = *reinterpret_cast<const float2*>(sec[tid]);
   auto publish_scales = [&] {
     if (tid < 32) {
-      mult[tid] = sec[tid] ? f.x * kCodeUnit<E4M3> : 1.f;
-      mult[32 + tid] = sec[tid] ? f.y * kCodeUnit<E4M3> : 1.f;
+      mult[tid] = sec[tid] ? f.x : 1.f;
+      mult[32 + tid] = sec[tid] ? f.y : 1.f;
     }
     named_bar_sync(1, kSealThreads<D>);   // reached from two places
   };

@@ -2,7 +2,8 @@
 // e4m3): append and sealing, reading back, attention, prefill staging and per-key attention weights.
 //
 // A page is one block. Pages that are complete and committed are sealed: x is held as q = round8(x / s), with
-// s = absmax / 127 (448 for e4m3; 1 for a block of zeros) over the page's 32 x D values of the head, K and V each.
+// s = absmax / 127 (448 for e4m3; 1 for a block of zeros) over the page's 32 x D values of the head, K and V each; an
+// int8 is stored as the byte q + 128.
 // The last tokens (an incomplete page, drafts that may be rolled back) stay in fp16 in a ring of 128 tokens per layer,
 // the tail, so a sealed page depends on committed tokens alone and a rollback needs no device work.
 //
@@ -86,7 +87,7 @@ __device__ __forceinline__ void encode16(const float (&v)[4][4], float scale, fl
     }
     return;
   }
-  constexpr float kMagic = 12582912.f;   // 1.5 * 2^23: adding it rounds to an integer, whose low byte is the code
+  constexpr float kMagic = 12582912.f + 128.f;   // 1.5 * 2^23: adding it rounds to an integer; the code is stored plus 128
   float t[4][4], worst = 0.f;
 #pragma unroll
   for (int k = 0; k < 4; ++k)
@@ -107,28 +108,29 @@ __device__ __forceinline__ void encode16(const float (&v)[4][4], float scale, fl
                        __byte_perm(__float_as_uint(t[k][2]), __float_as_uint(t[k][3]), 0x0040), 0x5410);
 }
 
-// Bytes 0, 1 (LO) or 2, 3 of a word of codes as an fp16 pair. int8: 0x64NN is 1024 + NN with NN = v ^ 0x80, minus
-// 1152. e4m3: sign and the 7 other bits moved to an fp16's sign and bits 13..7, which is the value times 2^-8 (the
-// exponent bias differs by 8; subnormals come out right), so the caller's scale carries the 2^8. Both are exact.
+// Bytes 0, 1 (or with HI 2, 3) of a word of codes as an fp16 pair, exactly. decode_raw is one instruction: the byte v + 128
+// of an int8 is, as the bits of a subnormal fp16, (v + 128) 2^-24; the unit goes into K's scale (kCodeUnit), and the
+// scores start from minus 128 times the row's sum of q. decode_pair gives the values: V's sums run over thousands of keys,
+// and with a bias of 128 in them the tensor cores' fp32 accumulation cost 8 times the error (0.0017 of the RMS over 131072).
+template <bool E4M3>
+constexpr float kCodeUnit = E4M3 ? 1.f : 0x1p24f;
+template <bool E4M3>
+constexpr float kCodeBias = E4M3 ? 0.f : 128.f * 0x1p-24f;
+template <bool E4M3, bool HI>
+__device__ __forceinline__ uint32_t decode_raw(uint32_t w) {
+  if (E4M3) {
+    uint32_t h;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)(HI ? w >> 16 : w)));
+    return h;
+  }
+  return __byte_perm(w, 0u, HI ? 0x4342 : 0x4140);
+}
 template <bool E4M3, bool HI>
 __device__ __forceinline__ uint32_t decode_pair(uint32_t w) {
-  if (E4M3) {
-    const uint32_t h = __byte_perm(w, 0u, HI ? 0x3424 : 0x1404);
-    return (h & 0x80008000u) | ((h >> 1) & 0x3f803f80u);
-  }
-  const uint32_t y = __byte_perm(w ^ 0x80808080u, 0x64u, HI ? 0x4342 : 0x4140);
-  __half2 v = *reinterpret_cast<const __half2*>(&y);
-  v = __hsub2(v, __floats2half2_rn(1152.f, 1152.f));
-  return *reinterpret_cast<uint32_t*>(&v);
-}
-template <bool E4M3>
-constexpr float kCodeUnit = E4M3 ? 256.f : 1.f;   // what decode_pair leaves to the scale
-
-// One code's value as fp32 (before the scale).
-template <bool E4M3>
-__device__ __forceinline__ float decode8(uint32_t byte) {
-  const float2 f = unpack_half2(decode_pair<E4M3, false>(byte));
-  return f.x * kCodeUnit<E4M3>;
+  if (E4M3) return decode_raw<E4M3, HI>(w);
+  const uint32_t h = __byte_perm(w, 0x64u, HI ? 0x4342 : 0x4140);   // 0x64NN: 1024 + NN
+  const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&h), __floats2half2_rn(1152.f, 1152.f));
+  return *reinterpret_cast<const uint32_t*>(&v);
 }
 
 __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
@@ -393,8 +395,8 @@ __global__ __launch_bounds__(128) void kv8_read_kernel(Kv8ReadArgs a) {
   __half* const v_out = a.v + h * D;
   if (t0 < a.sealed) {
     const char* sec = a.g.pool + phys_block(a.g, page) * a.g.block_bytes + h * a.g.head_bytes;
-    const float ks = reinterpret_cast<const float*>(sec)[0] * kCodeUnit<E4M3>;
-    const float vs = reinterpret_cast<const float*>(sec)[1] * kCodeUnit<E4M3>;
+    const float ks = reinterpret_cast<const float*>(sec)[0];
+    const float vs = reinterpret_cast<const float*>(sec)[1];
     const uint4* K = reinterpret_cast<const uint4*>(sec + S::kOffK);
     const uint32_t* V = reinterpret_cast<const uint32_t*>(sec + S::kOffV);
 #pragma unroll
@@ -508,18 +510,17 @@ __device__ __forceinline__ bool sees(int pos, int key, int window) {
 
 template <int D, int NT>
 struct Kv8Attn {
-  // 32 rows at head_dim 64 need about 160 registers: 12 warps in one block per SM; else 8 warps, two blocks per SM at
-  // head_dim 64 (ring and registers allow it), one at 128.
-  static constexpr bool kWide = D == 64 && NT == 4;
-  static constexpr int kWarps = kWide ? 12 : 8, kThreads = 32 * kWarps, kStages = kWide ? 4 : 3;
+  // Two blocks of 8 warps per SM at head_dim 64 (128 registers), one of 12 at 128 (168).
+  static constexpr int kWarps = D == 64 ? 8 : 12, kThreads = 32 * kWarps, kStages = D == 64 ? 3 : 2;
   static constexpr int kStageBytes = Q8Section<D>::kBytes;                 // a multiple of 32
   static constexpr int kRing = kWarps * kStages * kStageBytes;
   static constexpr int kOStride = D + 4;                                   // floats, 4 mod 32 banks
   static constexpr int kMerge = kWarps * 8 * NT * (kOStride + 2) * 4;      // over the ring once it is drained
   static constexpr int kOffQ = kRing > kMerge ? kRing : kMerge;
-  static constexpr int kOffBar = kOffQ + 8 * NT * D * 2;
+  static constexpr int kOffBias = kOffQ + 8 * NT * D * 2;                  // per row: - kCodeBias times the sum of q
+  static constexpr int kOffBar = kOffBias + 8 * NT * 4;
   static constexpr int kSmem = kOffBar + kWarps * kStages * 8;
-  static constexpr int kBlocksPerSm = D == 64 && !kWide ? 2 : 1;
+  static constexpr int kBlocksPerSm = D == 64 ? 2 : 1;
 };
 
 // Fragments of a tail page straight from the ring in global memory (fp16, L2-resident).
@@ -544,10 +545,243 @@ __device__ __forceinline__ uint32_t tail_v_pair(const TailView& t, int key, int 
   return w;
 }
 
+// -kCodeBias times the sum of each query row's values, by whole warps (order fixed).
+template <int D>
+__device__ __forceinline__ void stage_bias(const __half* q, int64_t q_stride, int rows, int group, int h, int row0, int count,
+                                           float bias, float* dst, int warp, int warps, int lane) {
+  for (int i = warp; i < count; i += warps) {
+    const int r = row0 + i;
+    float sum = 0.f;
+    if (r < rows) {
+      const int t = r / group, j = r - t * group;
+      const __half* src = q + t * q_stride + (int64_t)(h * group + j) * D;
+#pragma unroll
+      for (int k = 0; k < D / 64; ++k) {
+        const float2 f = unpack_half2(reinterpret_cast<const uint32_t*>(src)[lane + 32 * k]);
+        sum += f.x + f.y;
+      }
+    }
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) dst[i] = -bias * sum;
+  }
+}
+
+// d = a x b + (c0, c1, c0, c1).
+__device__ __forceinline__ void mma_f16_16816_from(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float2 c) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c.x), "f"(c.y));
+}
+
+// S^T of the HB 16-key halves of a sealed page and 8 NT query rows, by a warp: s[b][n] is an accumulator of keys
+// g, g + 8 (rows) and query rows 2 c, 2 c + 1 (columns). The accumulators start from the bias' share.
+template <int D, int NT, int HB, bool E4M3>
+struct Kv8Scores {
+  const uint8_t* k;      // the page's K codes
+  const uint4* sq;
+  const float* sbias;
+  int lane;
+  // The same scores, to be made anew: nothing of an earlier pass is kept in registers for it.
+  __device__ __forceinline__ Kv8Scores again() const {
+    Kv8Scores q = *this;
+    asm volatile("" : "+l"(q.k), "+l"(q.sq), "+l"(q.sbias));
+    return q;
+  }
+  __device__ __forceinline__ void operator()(float (&s)[HB][NT][4]) const {
+    constexpr int NE = D / 64;
+#pragma unroll
+    for (int e = 0; e < NE; ++e) {
+      uint32_t wa[HB][4], wb[HB][4];
+#pragma unroll
+      for (int b = 0; b < HB; ++b) {
+        const uint4* k4 = reinterpret_cast<const uint4*>(k) + (2 * b * NE + e) * 32 + lane;
+        const uint4 ra = k4[0], rb = k4[NE * 32];
+        wa[b][0] = ra.x;
+        wa[b][1] = ra.y;
+        wa[b][2] = ra.z;
+        wa[b][3] = ra.w;
+        wb[b][0] = rb.x;
+        wb[b][1] = rb.y;
+        wb[b][2] = rb.z;
+        wb[b][3] = rb.w;
+      }
+#pragma unroll
+      for (int s2 = 0; s2 < 2; ++s2) {
+        uint32_t f[HB][2][4];
+#pragma unroll
+        for (int b = 0; b < HB; ++b)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            f[b][u][0] = decode_raw<E4M3, false>(wa[b][2 * s2 + u]);
+            f[b][u][1] = decode_raw<E4M3, false>(wb[b][2 * s2 + u]);
+            f[b][u][2] = decode_raw<E4M3, true>(wa[b][2 * s2 + u]);
+            f[b][u][3] = decode_raw<E4M3, true>(wb[b][2 * s2 + u]);
+          }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const uint4 qv = sq[((n * NE + e) * 2 + s2) * 32 + lane];
+#pragma unroll
+          for (int b = 0; b < HB; ++b) {
+            if (e == 0 && s2 == 0) {
+              float2 start = make_float2(0.f, 0.f);
+              if (!E4M3) start = *reinterpret_cast<const float2*>(sbias + 8 * n + 2 * (lane & 3));
+              mma_f16_16816_from(s[b][n], f[b][0], qv.x, qv.y, start);
+            } else {
+              mma_f16_16816(s[b][n], f[b][0], qv.x, qv.y);
+            }
+            mma_f16_16816(s[b][n], f[b][1], qv.z, qv.w);
+          }
+        }
+      }
+    }
+  }
+};
+// The same for keys key0 .. of the tail (fp16).
+template <int D, int NT, int HB>
+struct Kv8TailScores {
+  TailView tail;
+  int key0;
+  const uint4* sq;
+  int lane;
+  __device__ __forceinline__ Kv8TailScores again() const {
+    Kv8TailScores q = *this;
+    asm volatile("" : "+l"(q.tail.k), "+l"(q.sq));
+    return q;
+  }
+  __device__ __forceinline__ void operator()(float (&s)[HB][NT][4]) const {
+    constexpr int NE = D / 64;
+#pragma unroll
+    for (int b = 0; b < HB; ++b) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[b][n][i] = 0.f;
+#pragma unroll
+      for (int e = 0; e < NE; ++e) {
+        uint2 kA[4], kB[4];
+        tail_k_frag<D>(tail, key0 + 16 * b, e, lane >> 2, lane & 3, kA, kB);
+#pragma unroll
+        for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            const uint4 qv = sq[((n * NE + e) * 2 + s2) * 32 + lane];
+            const uint32_t f0[4] = {kA[2 * s2].x, kB[2 * s2].x, kA[2 * s2].y, kB[2 * s2].y};
+            const uint32_t f1[4] = {kA[2 * s2 + 1].x, kB[2 * s2 + 1].x, kA[2 * s2 + 1].y, kB[2 * s2 + 1].y};
+            mma_f16_16816(s[b][n], f0, qv.x, qv.y);
+            mma_f16_16816(s[b][n], f1, qv.z, qv.w);
+          }
+      }
+    }
+  }
+};
+
+// x = x kc + off for one n-tile's scores, masked keys -inf (pos0, pos1: the positions of its rows 2 c and 2 c + 1).
+template <int NT, int HB>
+__device__ __forceinline__ void kv8_exponents(float (&x)[HB][NT][4], int n, float kc, float2 off, bool open, int pos0, int pos1,
+                                              int key, int window) {
+#pragma unroll
+  for (int b = 0; b < HB; ++b)
+#pragma unroll
+    for (int k = 0; k < 4; k += 2) {
+      const float2 e = ffma2(make_float2(x[b][n][k], x[b][n][k + 1]), make_float2(kc, kc), off);
+      x[b][n][k] = e.x;
+      x[b][n][k + 1] = e.y;
+    }
+  if (open) return;
+#pragma unroll
+  for (int b = 0; b < HB; ++b)
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      if (!sees(pos0, key + 16 * b + 8 * k, window)) x[b][n][2 * k] = -INFINITY;
+      if (!sees(pos1, key + 16 * b + 8 * k, window)) x[b][n][2 * k + 1] = -INFINITY;
+    }
+}
+
+// A warp's running state: O^T accumulators, the maxima of its lanes' rows, the sums of P' / vs, exact and with P' as rounded.
+template <int D, int NT>
+struct Kv8Rows {
+  float o[D / 16][NT][4];
+  float m[NT][2];
+  float2 l[NT], lp[NT];
+};
+
+// Softmax of HB x 16 keys from key0 on, P' packed as B operands. qk(x) makes the scores S^T; kc: their factor, lv: log2 of
+// the V scale, inv: its reciprocal. The scores become exponents in place; the rare page that moves a maximum makes them
+// again (keeping both spills at 16 rows and head_dim 64).
+template <int D, int NT, int HB, typename QK>
+__device__ __forceinline__ void kv8_softmax(const QK& qk, Kv8Rows<D, NT>& w, const Kv8AttnArgs& a, int row, int key0, bool open,
+                                            float kc, float lv, float inv, int lane, uint32_t (&pb)[HB][NT][2]) {
+  const int key = key0 + (lane >> 2);
+  float x[HB][NT][4];
+  qk(x);
+  float top = -INFINITY;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int r = row + 8 * n;
+    // +inf against a row without a maximum yet
+    kv8_exponents<NT, HB>(x, n, kc, make_float2(lv - w.m[n][0], lv - w.m[n][1]), open, open ? 0 : a.ctx_len + r / a.group,
+                          open ? 0 : a.ctx_len + (r + 1) / a.group, key, a.window);
+#pragma unroll
+    for (int b = 0; b < HB; ++b) top = fmax3(fmax3(top, x[b][n][0], x[b][n][1]), x[b][n][2], x[b][n][3]);
+  }
+  if (__any_sync(0xffffffffu, top > kLazy)) {
+    qk.again()(x);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int r = row + 8 * n;
+      kv8_exponents<NT, HB>(x, n, kc, make_float2(lv, lv), open, a.ctx_len + r / a.group, a.ctx_len + (r + 1) / a.group, key,
+                            a.window);
+      float f[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float mx = w.m[n][i];
+#pragma unroll
+        for (int b = 0; b < HB; ++b) mx = fmax3(mx, x[b][n][i], x[b][n][i + 2]);
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+        f[i] = mx == -INFINITY ? 1.f : fast_exp2(w.m[n][i] - mx);   // no key yet: 2^-inf = 0
+        w.m[n][i] = mx;
+        const float m = mx == -INFINITY ? 0.f : mx;
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d) {
+          w.o[d][n][i] *= f[i];
+          w.o[d][n][i + 2] *= f[i];
+        }
+#pragma unroll
+        for (int b = 0; b < HB; ++b) {
+          x[b][n][i] -= m;
+          x[b][n][i + 2] -= m;
+        }
+      }
+      w.l[n] = fmul2(w.l[n], make_float2(f[0], f[1]));
+      w.lp[n] = fmul2(w.lp[n], make_float2(f[0], f[1]));
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    float2 sum = make_float2(0.f, 0.f), rsum = sum;
+#pragma unroll
+    for (int b = 0; b < HB; ++b)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const float2 p = make_float2(fast_exp2(x[b][n][2 * k]), fast_exp2(x[b][n][2 * k + 1]));
+        const uint32_t hp = pack_half2(p.x, p.y);
+        sum = fadd2(sum, p);
+        rsum = fadd2(rsum, unpack_half2(hp));
+        pb[b][n][k] = movmatrix_trans(hp);
+      }
+    w.l[n] = ffma2(sum, make_float2(inv, inv), w.l[n]);
+    w.lp[n] = ffma2(rsum, make_float2(inv, inv), w.lp[n]);
+  }
+}
+
 // Attention of up to 8 NT query rows of one kv head over a split's pages. Grid (splits, kv heads, row groups).
 //
-// Each warp streams its own pages (every 8th of the split's) through its own ring of bulk copies, so no warp waits for
-// another before the end, and turns codes into fp16 operands in registers: Q, K and P V products are exact to fp32
+// Each warp streams its own pages (every kWarps-th of the split's) through its own ring of bulk copies, so no warp waits
+// for another before the end, and turns codes into fp16 operands in registers: Q, K and P V products are exact to fp32
 // accumulation, only P is rounded to fp16. Scores come as S^T (keys x rows), so the sealed pages' K scale is one factor
 // per page, and the V scale is folded into the exponent: P' = 2^(s + log2 vs - m'), with m' the running maximum of
 // s + log2 vs, gives sum P' v8 = 2^-m' sum 2^s v directly, and l = sum P' / vs is the softmax sum. m' is lazy (moved
@@ -558,15 +792,17 @@ template <int D, int NT, bool E4M3>
 __global__ __launch_bounds__(Kv8Attn<D, NT>::kThreads, Kv8Attn<D, NT>::kBlocksPerSm) void kv8_attend_kernel(Kv8AttnArgs a) {
   using L = Kv8Attn<D, NT>;
   using S = Q8Section<D>;
-  constexpr int NE = D / 64, W = L::kWarps, NS = L::kStages, NR = 8 * NT;
+  constexpr int W = L::kWarps, NS = L::kStages, NR = 8 * NT;
+  constexpr int HB = 2;   // both 16-key halves of a page together: independent MMA chains, one vote
   extern __shared__ __align__(1024) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const int h = blockIdx.y, split = blockIdx.x, row0 = blockIdx.z * NR, rows = a.m * a.group;
   const int kv_end = a.ctx_len + a.m;
   const int pg0 = a.p_begin + (int)((int64_t)a.p_total * split / a.splits);
   const int pg1 = a.p_begin + (int)((int64_t)a.p_total * (split + 1) / a.splits);
-  const int sealed_pages = a.sealed / kBlockTokens;
+  const int sealed_end = min(pg1, a.sealed / kBlockTokens);   // the split's sealed pages are [pg0, sealed_end)
   uint4* sq = reinterpret_cast<uint4*>(smem + L::kOffQ);
+  float* sbias = reinterpret_cast<float*>(smem + L::kOffBias);
   uint8_t* ring = smem + (size_t)warp * NS * L::kStageBytes;
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kOffBar) + warp * NS;
 
@@ -577,165 +813,77 @@ __global__ __launch_bounds__(Kv8Attn<D, NT>::kThreads, Kv8Attn<D, NT>::kBlocksPe
   __syncwarp();
   pdl_wait();
   const char* head = a.g.pool + h * a.g.head_bytes;
-  auto issue = [&](int page, int st) {
-    mbar_arrive_expect_tx(&full[st], L::kStageBytes);
-    bulk_g2s(ring + st * L::kStageBytes, head + phys_block(a.g, page) * a.g.block_bytes, L::kStageBytes, &full[st]);
-  };
   const int first = pg0 + warp;
-  int issued = 0, waited = 0;
-  if (lane == 0)
-    for (int p = first; issued < NS && p < pg1 && p < sealed_pages; p += W) issue(p, issued++);
-  issued = __shfl_sync(0xffffffffu, issued, 0);
+  const int npages = first < sealed_end ? (sealed_end - first + W - 1) / W : 0;   // this warp's sealed pages
+  // Block-table entries 32 of this warp's pages at a time, one per lane (a load per page would stall the warp).
+  int tab0 = 0;
+  int64_t entry = 0;
+  auto load_entries = [&] { entry = tab0 + lane < npages ? phys_block(a.g, first + (tab0 + lane) * W) : 0; };
+  load_entries();
+  int issued = 0;
+  auto issue = [&](int st) {
+    if (issued - tab0 == 32) {
+      tab0 += 32;
+      load_entries();
+    }
+    const int64_t blk = __shfl_sync(0xffffffffu, entry, issued - tab0);
+    if (lane == 0) {
+      mbar_arrive_expect_tx(&full[st], L::kStageBytes);
+      bulk_g2s(ring + st * L::kStageBytes, head + blk * a.g.block_bytes, L::kStageBytes, &full[st]);
+    }
+    ++issued;
+  };
+  while (issued < min(NS, npages)) issue(issued);
   stage_q<D>(a.q, a.q_stride, rows, a.group, h, row0, NT, sq, threadIdx.x, L::kThreads);
+  if (!E4M3)
+    stage_bias<D>(a.q, a.q_stride, rows, a.group, h, row0, NR, kCodeBias<E4M3>, sbias, warp, W, lane);
   __syncthreads();
 
-  float o[D / 16][NT][4];
-  float mr[NT][2];
-  float lr[NT][2], lp[NT][2];   // sums of P' / vs, exact and with P' as rounded to fp16
+  Kv8Rows<D, NT> w;
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      mr[n][i] = -INFINITY;
-      lr[n][i] = lp[n][i] = 0.f;
-    }
+    w.m[n][0] = w.m[n][1] = -INFINITY;
+    w.l[n] = w.lp[n] = make_float2(0.f, 0.f);
 #pragma unroll
     for (int d = 0; d < D / 16; ++d)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[d][n][i] = 0.f;
+      for (int i = 0; i < 4; ++i) w.o[d][n][i] = 0.f;
   }
 
   const TailView tail = tail_of(a.tail, a.g.kv_heads, h, D);
-  // Softmax of 16 keys (S^T in s) against this warp's rows, P' packed as B operands. kc: the scores' factor, lv: log2 of
-  // the V scale, inv: its reciprocal.
-  auto softmax16 = [&](float (&s)[NT][4], int key0, bool open, float kc, float lv, float inv, uint32_t (&pb)[NT][2]) {
-    if (!open) {
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int pos = a.ctx_len + (row0 + 8 * n + 2 * c + (i & 1)) / a.group;
-          if (!sees(pos, key0 + g + 8 * (i >> 1), a.window)) s[n][i] = -INFINITY;   // kc > 0 keeps it
-        }
-    }
-    float x[NT][4];
-    float top = -INFINITY;
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[n][i] = fmaf(s[n][i], kc, lv - mr[n][i & 1]);
-      // a masked score against a row without a maximum yet is -inf + inf: it stays masked
-      if (!open) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[n][i] = s[n][i] == -INFINITY ? -INFINITY : x[n][i];
-      }
-      top = fmaxf(fmax3(top, x[n][0], x[n][1]), fmaxf(x[n][2], x[n][3]));
-    }
-    if (__any_sync(0xffffffffu, top > kLazy)) {
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          float mx = fmaxf(fmaf(s[n][i], kc, lv), fmaf(s[n][i + 2], kc, lv));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-          mx = fmaxf(mx, mr[n][i]);
-          const float f = mx == -INFINITY ? 1.f : fast_exp2(mr[n][i] - mx);   // no key yet: 2^-inf = 0
-          mr[n][i] = mx;
-          lr[n][i] *= f;
-          lp[n][i] *= f;
-#pragma unroll
-          for (int d = 0; d < D / 16; ++d) {
-            o[d][n][i] *= f;
-            o[d][n][i + 2] *= f;
-          }
-          const float off = lv - (mx == -INFINITY ? 0.f : mx);
-          x[n][i] = fmaf(s[n][i], kc, off);
-          x[n][i + 2] = fmaf(s[n][i + 2], kc, off);
-        }
-    }
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      float p[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) p[i] = fast_exp2(x[n][i]);
-      const uint32_t h0 = pack_half2(p[0], p[1]), h1 = pack_half2(p[2], p[3]);
-      const float2 r = fadd2(unpack_half2(h0), unpack_half2(h1));
-      lr[n][0] = fmaf(p[0] + p[2], inv, lr[n][0]);
-      lr[n][1] = fmaf(p[1] + p[3], inv, lr[n][1]);
-      lp[n][0] = fmaf(r.x, inv, lp[n][0]);
-      lp[n][1] = fmaf(r.y, inv, lp[n][1]);
-      pb[n][0] = movmatrix_trans(h0);
-      pb[n][1] = movmatrix_trans(h1);
-    }
-  };
-
   bool ok = true;
-  int st = 0, next = first + issued * W;
+  int st = 0, waited = 0;
   uint32_t phase = 0;
-  for (int page = first; page < pg1 && page < sealed_pages; page += W) {
+#pragma unroll 1
+  for (; waited < npages;) {
     ok = __all_sync(0xffffffffu, mbar_wait(&full[st], phase));
     if (!ok) break;
+    const int page = first + waited * W;
     ++waited;
     const uint8_t* sec = ring + st * L::kStageBytes;
-    const float ks = reinterpret_cast<const float*>(sec)[0], vs = reinterpret_cast<const float*>(sec)[1];
-    const float kc = ks * kCodeUnit<E4M3> * a.qk_scale, vu = vs * kCodeUnit<E4M3>;
-    const float lv = __log2f(vu), inv = __fdividef(1.f, vu);
+    const float vs = reinterpret_cast<const float*>(sec)[1];
+    const float kc = reinterpret_cast<const float*>(sec)[0] * kCodeUnit<E4M3> * a.qk_scale, lv = __log2f(vs), inv = __fdividef(1.f, vs);
     const bool open = page_open(page, a.ctx_len, a.m, a.window);
+    const Kv8Scores<D, NT, HB, E4M3> qk{sec + S::kOffK, sq, sbias, lane};
+    uint32_t pb[HB][NT][2];
+    kv8_softmax<D, NT, HB>(qk, w, a, row0 + 2 * c, page * kBlockTokens, open, kc, lv, inv, lane, pb);
 #pragma unroll
-    for (int mt = 0; mt < 2; ++mt) {
-      float s[NT][4];
+    for (int d = 0; d < D / 32; ++d)
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s[n][i] = 0.f;
-      const uint4* kc4 = reinterpret_cast<const uint4*>(sec + S::kOffK) + (mt * 2 * NE) * 32 + lane;
-#pragma unroll
-      for (int e = 0; e < NE; ++e) {
-        const uint4 ra = kc4[e * 32], rb = kc4[(NE + e) * 32];
-        const uint32_t wa[4] = {ra.x, ra.y, ra.z, ra.w}, wb[4] = {rb.x, rb.y, rb.z, rb.w};
-#pragma unroll
-        for (int s2 = 0; s2 < 2; ++s2) {
-          uint32_t fa[2][4];
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            fa[u][0] = decode_pair<E4M3, false>(wa[2 * s2 + u]);
-            fa[u][1] = decode_pair<E4M3, false>(wb[2 * s2 + u]);
-            fa[u][2] = decode_pair<E4M3, true>(wa[2 * s2 + u]);
-            fa[u][3] = decode_pair<E4M3, true>(wb[2 * s2 + u]);
-          }
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            const uint4 qv = sq[((n * NE + e) * 2 + s2) * 32 + lane];
-            mma_f16_16816(s[n], fa[0], qv.x, qv.y);
-            mma_f16_16816(s[n], fa[1], qv.z, qv.w);
-          }
-        }
-      }
-      uint32_t pb[NT][2];
-      softmax16(s, page * kBlockTokens + 16 * mt, open, kc, lv, inv, pb);
-      const uint4* vc4 = reinterpret_cast<const uint4*>(sec + S::kOffV) + mt * (D / 32) * 32 + lane;
-#pragma unroll
-      for (int d = 0; d < D / 32; ++d) {
-        const uint4 r = vc4[d * 32];
+      for (int b = 0; b < HB; ++b) {
+        const uint4 r = reinterpret_cast<const uint4*>(sec + S::kOffV)[(b * (D / 32) + d) * 32 + lane];
         const uint32_t f0[4] = {decode_pair<E4M3, false>(r.x), decode_pair<E4M3, false>(r.y),
                                 decode_pair<E4M3, true>(r.x), decode_pair<E4M3, true>(r.y)};
         const uint32_t f1[4] = {decode_pair<E4M3, false>(r.z), decode_pair<E4M3, false>(r.w),
                                 decode_pair<E4M3, true>(r.z), decode_pair<E4M3, true>(r.w)};
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          mma_f16_16816(o[2 * d][n], f0, pb[n][0], pb[n][1]);
-          mma_f16_16816(o[2 * d + 1][n], f1, pb[n][0], pb[n][1]);
+          mma_f16_16816(w.o[2 * d][n], f0, pb[b][n][0], pb[b][n][1]);
+          mma_f16_16816(w.o[2 * d + 1][n], f1, pb[b][n][0], pb[b][n][1]);
         }
       }
-    }
     __syncwarp();   // every lane has read the stage
-    if (next < pg1 && next < sealed_pages) {
-      if (lane == 0) issue(next, st);
-      ++issued;
-    }
-    next += W;
+    if (issued < npages) issue(st);
     if (++st == NS) {
       st = 0;
       phase ^= 1;
@@ -752,66 +900,42 @@ __global__ __launch_bounds__(Kv8Attn<D, NT>::kThreads, Kv8Attn<D, NT>::kBlocksPe
     }
   }
   // Tail pages (fp16): the first one of this warp's at or past the sealed ones.
-  int page = first;
-  if (page < sealed_pages) page += (sealed_pages - page + W - 1) / W * W;
-  for (; page < pg1; page += W) {
 #pragma unroll 1
-    for (int mt = 0; mt < 2; ++mt) {
-      const int key0 = page * kBlockTokens + 16 * mt;
-      if (key0 >= kv_end) break;
-      float s[NT][4];
+  for (int page = first + npages * W; page < pg1; page += W) {
+    const int key0 = page * kBlockTokens;
+    const Kv8TailScores<D, NT, HB> qk{tail, key0, sq, lane};
+    uint32_t pb[HB][NT][2];
+    kv8_softmax<D, NT, HB>(qk, w, a, row0 + 2 * c, key0, false, a.qk_scale, 0.f, 1.f, lane, pb);
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s[n][i] = 0.f;
-#pragma unroll
-      for (int e = 0; e < NE; ++e) {
-        uint2 kA[4], kB[4];
-        tail_k_frag<D>(tail, key0, e, g, c, kA, kB);
-#pragma unroll
-        for (int s2 = 0; s2 < 2; ++s2)
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            const uint4 qv = sq[((n * NE + e) * 2 + s2) * 32 + lane];
-            const uint32_t f0[4] = {kA[2 * s2].x, kB[2 * s2].x, kA[2 * s2].y, kB[2 * s2].y};
-            const uint32_t f1[4] = {kA[2 * s2 + 1].x, kB[2 * s2 + 1].x, kA[2 * s2 + 1].y, kB[2 * s2 + 1].y};
-            mma_f16_16816(s[n], f0, qv.x, qv.y);
-            mma_f16_16816(s[n], f1, qv.z, qv.w);
-          }
-      }
-      uint32_t pb[NT][2];
-      softmax16(s, key0, false, a.qk_scale, 0.f, 1.f, pb);
-      const int k0 = key0 + 2 * c;
+    for (int b = 0; b < HB; ++b) {
+      const int k0 = key0 + 16 * b + 2 * c;
 #pragma unroll
       for (int d = 0; d < D / 16; ++d) {
         const int dim = 16 * d + g;
         const uint32_t f[4] = {tail_v_pair(tail, k0, dim, kv_end), tail_v_pair(tail, k0, dim + 8, kv_end),
                                tail_v_pair(tail, k0 + 8, dim, kv_end), tail_v_pair(tail, k0 + 8, dim + 8, kv_end)};
 #pragma unroll
-        for (int n = 0; n < NT; ++n) mma_f16_16816(o[d][n], f, pb[n][0], pb[n][1]);
+        for (int n = 0; n < NT; ++n) mma_f16_16816(w.o[d][n], f, pb[b][n][0], pb[b][n][1]);
       }
     }
   }
 
   // The warps' rows meet in shared memory: [warp][row][D + 4] acc, then [warp][row] (max, sum).
 #pragma unroll
-  for (int n = 0; n < NT; ++n)
+  for (int n = 0; n < NT; ++n) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-#pragma unroll
-      for (int x = 4; x <= 16; x <<= 1) {
-        lr[n][i] += __shfl_xor_sync(0xffffffffu, lr[n][i], x);
-        lp[n][i] += __shfl_xor_sync(0xffffffffu, lp[n][i], x);
-      }
-      // acc / lp is the mean over P' as rounded (numerator and denominator carry the same roundings); from here on
-      // acc is relative to the exact sum, which the log-sum-exp needs
-      const float f = lp[n][i] > 0.f ? lr[n][i] / lp[n][i] : 1.f;
-#pragma unroll
-      for (int d = 0; d < D / 16; ++d) {
-        o[d][n][i] *= f;
-        o[d][n][i + 2] *= f;
-      }
+    for (int x = 4; x <= 16; x <<= 1) {
+      w.l[n] = fadd2(w.l[n], make_float2(__shfl_xor_sync(0xffffffffu, w.l[n].x, x), __shfl_xor_sync(0xffffffffu, w.l[n].y, x)));
+      w.lp[n] = fadd2(w.lp[n], make_float2(__shfl_xor_sync(0xffffffffu, w.lp[n].x, x), __shfl_xor_sync(0xffffffffu, w.lp[n].y, x)));
     }
+    // acc / lp is the mean over P' as rounded (numerator and denominator carry the same roundings); from here on acc is
+    // relative to the exact sum, which the log-sum-exp needs
+    const float f[2] = {w.lp[n].x > 0.f ? w.l[n].x / w.lp[n].x : 1.f, w.lp[n].y > 0.f ? w.l[n].y / w.lp[n].y : 1.f};
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w.o[d][n][i] *= f[i & 1];
+  }
   __syncthreads();   // the rings are drained
   float* so = reinterpret_cast<float*>(smem);
   float2* sm = reinterpret_cast<float2*>(smem + W * NR * L::kOStride * 4);
@@ -823,10 +947,10 @@ __global__ __launch_bounds__(Kv8Attn<D, NT>::kThreads, Kv8Attn<D, NT>::kBlocksPe
       float* dst = so + (warp * NR + r) * L::kOStride + g;
 #pragma unroll
       for (int d = 0; d < D / 16; ++d) {
-        dst[16 * d] = o[d][n][i];
-        dst[16 * d + 8] = o[d][n][i + 2];
+        dst[16 * d] = w.o[d][n][i];
+        dst[16 * d + 8] = w.o[d][n][i + 2];
       }
-      if (g == 0) sm[warp * NR + r] = make_float2(mr[n][i], lr[n][i]);
+      if (g == 0) sm[warp * NR + r] = make_float2(w.m[n][i], i ? w.l[n].y : w.l[n].x);
     }
   }
   __syncthreads();
@@ -862,39 +986,56 @@ __global__ __launch_bounds__(Kv8Attn<D, NT>::kThreads, Kv8Attn<D, NT>::kBlocksPe
   }
 }
 
-// Merge of a row's split partials (acc[D], max, sum): one block of 128 threads per row, thread = (pair of dims, group
-// of splits), each thread's loads independent; the weights 2^(m - M) in shared memory.
-constexpr int kKv8CombineThreads = 128, kKv8MaxSplits = 1024;
+// Merge of a row's split partials (acc[D], max, sum): one block of 2 D threads per row, thread = (pair of dims, quarter of
+// the splits). The loads of 64 splits go out at once (a lane of each warp holds (max, sum) of two splits): one round trip
+// to L2 where maxima, sums and accumulators one after the other took three. More splits go 64 at a time.
+constexpr int kKv8MaxSplits = 1024;
 template <int D>
-__global__ __launch_bounds__(kKv8CombineThreads) void kv8_combine_kernel(const float* part, int splits, const __half* gate,
-                                                                         __half* out, float* lse) {
-  constexpr int P = D / 2, G = kKv8CombineThreads / P;
-  __shared__ float w[kKv8MaxSplits];
-  __shared__ float red[32];
+__global__ __launch_bounds__(2 * D, 4) void kv8_combine_kernel(const float* part, int splits, const __half* gate, __half* out,
+                                                            float* lse) {
+  constexpr int P = D / 2, G = 4, U = 64 / G;
   __shared__ float2 acc[G][P];
   pdl_wait();
   pdl_trigger();
-  const int row = blockIdx.x, tid = threadIdx.x, p = tid % P, gi = tid / P;
+  const int row = blockIdx.x, tid = threadIdx.x, p = tid % P, gi = tid / P, lane = tid & 31;   // a warp has one gi
   const float* base = part + (int64_t)row * splits * (D + 2);
-  float mx = -INFINITY;
-  for (int s = tid; s < splits; s += kKv8CombineThreads) {
-    w[s] = base[(int64_t)s * (D + 2) + D];
-    mx = fmaxf(mx, w[s]);
-  }
-  mx = block_reduce(mx, true, red);
-  float l = 0.f;
-  for (int s = tid; s < splits; s += kKv8CombineThreads) {
-    const float f = w[s] == -INFINITY ? 0.f : fast_exp2(w[s] - mx);
-    l = fmaf(f, base[(int64_t)s * (D + 2) + D + 1], l);
-    w[s] = f;
-  }
-  l = block_reduce(l, false, red);   // its barriers also publish w
+  float M = -INFINITY, l = 0.f;
   float2 x = make_float2(0.f, 0.f);
-#pragma unroll 8
-  for (int s = gi; s < splits; s += G) {
-    const float2 v = *reinterpret_cast<const float2*>(base + (int64_t)s * (D + 2) + 2 * p);
-    x.x = fmaf(w[s], v.x, x.x);
-    x.y = fmaf(w[s], v.y, x.y);
+  for (int s0 = 0; s0 < splits; s0 += 64) {
+    float2 ml[2], v[U];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int s = s0 + lane + 32 * k;
+      ml[k] = s < splits ? *reinterpret_cast<const float2*>(base + (int64_t)s * (D + 2) + D) : make_float2(-INFINITY, 0.f);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {   // splits U gi + u of the 64
+      const int s = s0 + U * gi + u;
+      v[u] = s < splits ? *reinterpret_cast<const float2*>(base + (int64_t)s * (D + 2) + 2 * p) : make_float2(0.f, 0.f);
+    }
+    float m = fmaxf(ml[0].x, ml[1].x);
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    m = fmaxf(m, M);
+    const float old = M == -INFINITY ? 0.f : fast_exp2(M - m);
+    M = m;
+    float w[2], sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      w[k] = ml[k].x == -INFINITY ? 0.f : fast_exp2(ml[k].x - m);
+      sum = fmaf(w[k], ml[k].y, sum);
+    }
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    l = fmaf(l, old, sum);
+    x.x *= old;
+    x.y *= old;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {   // all of a warp's splits lie in one half of the 64
+      const float f = __shfl_sync(0xffffffffu, gi < G / 2 ? w[0] : w[1], (U * gi + u) & 31);
+      x.x = fmaf(f, v[u].x, x.x);
+      x.y = fmaf(f, v[u].y, x.y);
+    }
   }
   acc[gi][p] = x;
   __syncthreads();
@@ -906,7 +1047,7 @@ __global__ __launch_bounds__(kKv8CombineThreads) void kv8_combine_kernel(const f
     }
     const float scale = (l > 0.f ? 1.f / l : 0.f) * sigmoid_gate(gate, row);
     *reinterpret_cast<uint32_t*>(out + (int64_t)row * D + 2 * p) = pack_half2(x.x * scale, x.y * scale);
-    if (lse && p == 0) lse[row] = (mx + log2f(l)) * kLn2;
+    if (lse && p == 0) lse[row] = (M + log2f(l)) * kLn2;
   }
 }
 
@@ -940,8 +1081,8 @@ __global__ __launch_bounds__(128) void kv8_expand_kernel(Kv8ExpandArgs a) {
   if (t0 < a.sealed) {
     const char* sec = a.g.pool + phys_block(a.g, page) * a.g.block_bytes + h * a.g.head_bytes;
     if (tid == 0) {
-      const float ks = reinterpret_cast<const float*>(sec)[0] * kCodeUnit<E4M3>;
-      const float vs = reinterpret_cast<const float*>(sec)[1] * kCodeUnit<E4M3>;
+      const float ks = reinterpret_cast<const float*>(sec)[0];
+      const float vs = reinterpret_cast<const float*>(sec)[1];
       a.scales[section] = make_float4(ks, log2f(vs), 1.f / vs, 0.f);
     }
     // Tile rows of 16 bytes: 8 dims of one key (K), 8 keys of one dim (V).
@@ -1006,7 +1147,8 @@ struct Kv8Weights {
   static constexpr int kRing = kWarps * kStages * kStageBytes;
   static constexpr int kMaxRows = 256;
   static __host__ __device__ constexpr int lse_off(int ntiles) { return kRing + ntiles * 8 * D * 2; }
-  static __host__ __device__ constexpr int bar_off(int ntiles) { return lse_off(ntiles) + ntiles * 8 * 4; }
+  static __host__ __device__ constexpr int bias_off(int ntiles) { return lse_off(ntiles) + ntiles * 8 * 4; }
+  static __host__ __device__ constexpr int bar_off(int ntiles) { return bias_off(ntiles) + ntiles * 8 * 4; }
   static __host__ __device__ constexpr int smem(int ntiles) { return bar_off(ntiles) + kWarps * kStages * 8; }
 };
 
@@ -1027,6 +1169,7 @@ __global__ __launch_bounds__(Kv8Weights<D>::kThreads, 2) void kv8_weights_kernel
   const int sealed_pages = a.sealed / kBlockTokens;
   uint4* sq = reinterpret_cast<uint4*>(smem + L::kRing);
   float* slse = reinterpret_cast<float*>(smem + L::lse_off(ntiles));
+  float* sbias = reinterpret_cast<float*>(smem + L::bias_off(ntiles));
   uint8_t* ring = smem + (size_t)warp * NS * L::kStageBytes;
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::bar_off(ntiles)) + warp * NS;
 
@@ -1047,6 +1190,7 @@ __global__ __launch_bounds__(Kv8Weights<D>::kThreads, 2) void kv8_weights_kernel
     for (int p = first; issued < NS && p < pg1 && p < sealed_pages; p += W) issue(p, issued++);
   issued = __shfl_sync(0xffffffffu, issued, 0);
   stage_q<D>(a.q, a.q_stride, rows, a.group, h, 0, ntiles, sq, threadIdx.x, L::kThreads);
+  if (!E4M3) stage_bias<D>(a.q, a.q_stride, rows, a.group, h, 0, 8 * ntiles, kCodeBias<E4M3>, sbias, warp, W, lane);
   for (int r = threadIdx.x; r < 8 * ntiles; r += L::kThreads) {
     const int t = r / a.group, j = r - t * a.group;
     // a padding row, and a row that saw no key (lse -inf), weighs nothing
@@ -1057,11 +1201,13 @@ __global__ __launch_bounds__(Kv8Weights<D>::kThreads, 2) void kv8_weights_kernel
 
   const TailView tail = tail_of(a.tail, a.g.kv_heads, h, D);
   // The page's 32 keys against all rows; lane i adds key i's sum to old and stores it.
-  auto rows32 = [&](const uint32_t (&f)[2][4 * NE][4], int page, bool open, float kc, float old) {
+  auto rows32 = [&](const uint32_t (&f)[2][4 * NE][4], int page, bool open, float kc, float old, bool biased) {
     float w[4] = {0.f, 0.f, 0.f, 0.f};   // keys 8 i + g
 #pragma unroll 2
     for (int n = 0; n < ntiles; ++n) {
-      float s[2][4] = {};
+      float2 bias = make_float2(0.f, 0.f);
+      if (!E4M3 && biased) bias = *reinterpret_cast<const float2*>(sbias + 8 * n + 2 * c);
+      float s[2][4] = {{bias.x, bias.y, bias.x, bias.y}, {bias.x, bias.y, bias.x, bias.y}};
 #pragma unroll
       for (int e = 0; e < 2 * NE; ++e) {
         const uint4 qv = sq[(n * 2 * NE + e) * 32 + lane];
@@ -1126,14 +1272,14 @@ __global__ __launch_bounds__(Kv8Weights<D>::kThreads, 2) void kv8_weights_kernel
         const uint32_t wa[4] = {ra.x, ra.y, ra.z, ra.w}, wb[4] = {rb.x, rb.y, rb.z, rb.w};
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-          f[mt][4 * e + u][0] = decode_pair<E4M3, false>(wa[u]);
-          f[mt][4 * e + u][1] = decode_pair<E4M3, false>(wb[u]);
-          f[mt][4 * e + u][2] = decode_pair<E4M3, true>(wa[u]);
-          f[mt][4 * e + u][3] = decode_pair<E4M3, true>(wb[u]);
+          f[mt][4 * e + u][0] = decode_raw<E4M3, false>(wa[u]);
+          f[mt][4 * e + u][1] = decode_raw<E4M3, false>(wb[u]);
+          f[mt][4 * e + u][2] = decode_raw<E4M3, true>(wa[u]);
+          f[mt][4 * e + u][3] = decode_raw<E4M3, true>(wb[u]);
         }
       }
     }
-    rows32(f, page, open, kc, old);
+    rows32(f, page, open, kc, old, true);
     __syncwarp();
     if (next < pg1 && next < sealed_pages) {
       if (lane == 0) issue(next, st);
@@ -1173,7 +1319,7 @@ __global__ __launch_bounds__(Kv8Weights<D>::kThreads, 2) void kv8_weights_kernel
           f[mt][4 * e + u][3] = kB[u].y;
         }
       }
-    rows32(f, page, false, a.qk_scale, load_prev(page));
+    rows32(f, page, false, a.qk_scale, load_prev(page), false);
   }
 }
 

@@ -17,6 +17,7 @@
 #include "i8rec.cuh"
 #include "kv.cuh"
 #include "kv8.cuh"
+#include "kv8tc.cuh"
 #include "module.cuh"
 #include "pcache.h"
 #include "prefill.cuh"
@@ -1217,17 +1218,18 @@ int with_format(const lfm3a_kv_layout& L, F f) {
   return e4m3 ? f(std::integral_constant<int, 128>{}, std::true_type{}) : f(std::integral_constant<int, 128>{}, std::false_type{});
 }
 
-int kv8_rows_per_group(int rows) { return rows <= 8 ? 8 : rows <= 16 ? 16 : 32; }
+// Query rows of one kv head that a block takes: kv8_attend_kernel's 8 or 16, or the 64 of kv8_attend_tc_kernel. 17 to 32 rows
+// go through the former in two groups: over 131072 tokens at 32/8/64 (int8) 52.7 us against 60.4; 48 rows 72 against 61,
+// 64 rows 91 against 62, 128 rows 191 against 111.
+int kv8_rows_per_block(int rows) { return rows <= 8 ? 8 : rows <= 32 ? 16 : 64; }
 
-// Key splits of kv8_attend_kernel: whole waves of its resident blocks (two per SM at head_dim 64, one at 128), at least
-// a page for each of a block's warps.
+// Key splits: one wave of resident blocks, at least a page for each of a block's warps (8, 12 at head_dim 128), or a
+// 128-key tile.
 int kv8_splits_for(int kv_heads, int head_dim, int rows, int pages, int sm_count) {
-  const int groups = kv_heads * ((rows + kv8_rows_per_group(rows) - 1) / kv8_rows_per_group(rows));
-  const int nr = kv8_rows_per_group(rows);
-  const bool wide = head_dim == 64 && nr == 32;
-  const int target = (head_dim == 64 && !wide ? 2 : 1) * sm_count, warps = wide ? 12 : 8;
-  const int splits = std::max(1, target / groups);
-  return std::min(std::min(splits, std::max(1, (pages + warps - 1) / warps)), kKv8MaxSplits);
+  const int nr = kv8_rows_per_block(rows), groups = kv_heads * ((rows + nr - 1) / nr);
+  const int per_sm = nr < 64 && head_dim == 64 ? 2 : 1, least = nr == 64 ? 4 : head_dim == 64 ? 8 : 12;
+  const int splits = std::max(1, per_sm * sm_count / groups);
+  return std::min(std::min(splits, std::max(1, (pages + least - 1) / least)), kKv8MaxSplits);
 }
 
 int kv8_pages(int ctx_len, int m, int window, int* begin) {
@@ -1359,7 +1361,9 @@ int lfm3a_kv8_attention(const lfm3a_kv8_view* kv, const void* q, int64_t q_strid
   a.qk_scale = (1.f / sqrtf((float)D)) * kLog2e;
   const int rows = m * group;
   if (splits <= 0) splits = kv8_splits_for(H, D, rows, a.p_total, current_sm_count());
-  a.splits = std::min(std::min(splits, a.p_total), kKv8MaxSplits);
+  // No split without a page (or a tile of four).
+  const int units = kv8_rows_per_block(rows) < 64 ? a.p_total : (a.p_begin + a.p_total - 1) / 4 - a.p_begin / 4 + 1;
+  a.splits = std::min(std::min(splits, units), kKv8MaxSplits);
   a.part = nullptr;
   if (a.splits > 1) {
     if (!workspace || !aligned16(workspace)) return fail(LFM3A_EINVAL, "kv8 attention needs a 16-byte aligned workspace");
@@ -1369,7 +1373,7 @@ int lfm3a_kv8_attention(const lfm3a_kv8_view* kv, const void* q, int64_t q_strid
   }
   const cudaStream_t st = as_stream(stream);
   static std::atomic<bool> done[12][64];
-  const int nr = kv8_rows_per_group(rows);
+  const int nr = kv8_rows_per_block(rows);
   const dim3 grid(a.splits, H, (rows + nr - 1) / nr);
   rc = with_format(L, [&](auto d, auto f) {
     constexpr int DD = decltype(d)::value;
@@ -1382,13 +1386,13 @@ int lfm3a_kv8_attention(const lfm3a_kv8_view* kv, const void* q, int64_t q_strid
     };
     if (nr == 8) return run(kv8_attend_kernel<DD, 1, E>, Kv8Attn<DD, 1>::kSmem, Kv8Attn<DD, 1>::kThreads, 0);
     if (nr == 16) return run(kv8_attend_kernel<DD, 2, E>, Kv8Attn<DD, 2>::kSmem, Kv8Attn<DD, 2>::kThreads, 1);
-    return run(kv8_attend_kernel<DD, 4, E>, Kv8Attn<DD, 4>::kSmem, Kv8Attn<DD, 4>::kThreads, 2);
+    return run(kv8_attend_tc_kernel<DD, E>, Kv8Tc<DD>::kSmem, kTcThreads, 2);
   });
   if (rc != LFM3A_OK) return rc;
   rc = check_launch("kv8_attend_kernel");
   if (rc != LFM3A_OK || a.splits == 1) return rc;
-  if (D == 64) launch_pdl(kv8_combine_kernel<64>, m * q_heads, kKv8CombineThreads, 0, st, a.part, a.splits, a.gate, a.out, lse);
-  else launch_pdl(kv8_combine_kernel<128>, m * q_heads, kKv8CombineThreads, 0, st, a.part, a.splits, a.gate, a.out, lse);
+  if (D == 64) launch_pdl(kv8_combine_kernel<64>, m * q_heads, 128, 0, st, a.part, a.splits, a.gate, a.out, lse);
+  else launch_pdl(kv8_combine_kernel<128>, m * q_heads, 256, 0, st, a.part, a.splits, a.gate, a.out, lse);
   return check_launch("kv8_combine_kernel");
 }
 

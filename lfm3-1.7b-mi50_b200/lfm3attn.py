@@ -645,13 +645,14 @@ def evict_select(weights, length: int, budget: int, sink: int, recent: int, stre
     """(keep int32 [kv_heads][budget] ascending, the kept keys' weights fp32) of weights fp32 [kv_heads][>= length]."""
     import torch
 
-    h = weights.shape[0]
-    if weights.dtype != torch.float32 or weights.shape[1] < length or weights.stride(1) != 1:
+    h, width = weights.shape
+    row, one = weights.stride()
+    if weights.dtype != torch.float32 or width < length or one != 1:
         raise LFM3AError(EINVAL, "weights must be fp32 [kv_heads][>= length]")
-    keep = torch.empty((h, max(0, budget)), dtype=torch.int32, device=weights.device)
-    kept = torch.empty((h, max(0, budget)), dtype=torch.float32, device=weights.device)
-    _check(lib().lfm3a_evict_select(_ptr(weights), weights.stride(0), h, length, sink, recent, budget, _ptr(keep),
-                                    _ptr(kept), kept.stride(0), _stream(stream)))
+    kept = weights.new_empty((h, max(0, budget)))
+    keep = torch.empty_like(kept, dtype=torch.int32)
+    _check(lib().lfm3a_evict_select(weights.data_ptr(), row, h, length, sink, recent, budget, keep.data_ptr(),
+                                    kept.data_ptr(), kept.stride(0), _stream(stream)))
     return keep, kept
 
 

@@ -47,7 +47,7 @@ def quantise(x, fmt):
     y = (x.astype(np.float32) / scale).astype(np.float32)
     if fmt == "int8":
         c = np.clip(np.rint(y), -127, 127).astype(np.int8)
-        return c.view(np.uint8), c.astype(np.float32), scale
+        return c.view(np.uint8) ^ 0x80, c.astype(np.float32), scale   # stored plus 128
     t = torch.from_numpy(np.clip(y, -448, 448)).to(torch.float8_e4m3fn)
     return t.view(torch.uint8).numpy(), t.float().numpy(), scale
 
