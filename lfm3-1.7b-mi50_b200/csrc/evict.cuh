@@ -33,7 +33,9 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 // the warps write the kept positions in order, each starting where the counts of the warps and blocks before it end. Of
 // keys equal to the last one kept the first ones stay, so the result does not depend on any order of execution. The keys
 // stay in shared memory up to 49152 per block; a longer share is read again (L2) on each sweep. The sweeps are short
-// loops: unrolled over registers they were slower, each instruction being fetched for one use.
+// loops: unrolled over registers they were slower, each instruction being fetched for one use. Bound by the latency of its
+// steps: 8 heads x 131072 positions take 22.6 us, of which a pass with its cluster barrier is 2.6 (1.9 at 20000), 4 x 5003
+// 8.0 us, 8 x 1000 4.9 us.
 template <int C>
 __device__ __forceinline__ void evict_select(const EvictArgs& a) {
   namespace cg = cooperative_groups;
@@ -203,7 +205,7 @@ struct Kv8CompactArgs {
 // No value passes through shared memory: a thread makes one chunk of the new page, of K (16 dims of a token, one chunk
 // of the old one) or of V (4 dims of 4 tokens: a byte from each word of a chunk of each token's page), and holds it as
 // fp16 codes while the block finds the scale. (Staged in shared memory as values it took 67 us for 8 x 32768 of 131072
-// tokens, bound by instructions.)
+// tokens, bound by instructions; this takes 36 us, 3.5 TB/s of sectors.)
 template <int D, bool E4M3>
 __global__ __launch_bounds__(kSealThreads<D>) void kv8_compact_kernel(Kv8CompactArgs a) {
   using S = Q8Section<D>;

@@ -1,4 +1,4 @@
-// Attention over the 8-bit block cache on tcgen05, for calls with more than 16 query rows per kv head (kv8.cuh has the
+// Attention over the 8-bit block cache on tcgen05, for calls with more than 32 query rows per kv head (kv8.cuh has the
 // cache's layout and the warp-level kernel for fewer).
 //
 // A CTA takes up to 64 query rows (r = t * group + j) of one kv head and a run of 128-key tiles (4 pages). The tensor
@@ -10,10 +10,16 @@
 //   the waits between them.)
 // S = Q K^T as in verify.cuh: M = 64 accumulators, the tile's two 64-key halves at lane offsets 0 and 16, so a lane
 // scores 64 keys (two pages) of one row and no lane is padding. With one factor per page, a lane needs two multipliers
-// for its 64 scores; the V scale goes into the exponent (see kv8_attend_kernel). Each (warpgroup, half) keeps its own
-// running (max, sum, O); the four streams meet at the end. With the two warpgroups on alternate tiles one's TMEM loads,
-// maxima and stores run beside the other's exponentials, which are the bound: 64 x 128 per tile at 16 a cycle are 512
-// of the 710 cycles the tile's 16.5 KB take from HBM.
+// for its 64 scores; the V scale goes into the exponent (see kv8_softmax). Each (warpgroup, half) keeps its own running
+// (max, sum, O); the four streams meet at the end. With the two warpgroups on alternate tiles one's TMEM loads, maxima
+// and stores run beside the other's exponentials.
+//
+// What bounds it: a tile (16.5 KB, 710 cycles of an SM's share of HBM) takes about 1700 cycles at head_dim 64. A timeline
+// of one CTA puts 1850 on a warpgroup's softmax of every other tile, 1300-1600 on a converter's tile, 8 MMAs of some 70
+// cycles on each issuing warp, all on 4.5 warps per scheduler; shared memory alone moves 144 KB a tile, 1150 cycles (codes
+// in, codes out, fp16 in, operands out). The warp-level kernel converts in registers and has no such traffic, but its
+// MMAs (8 cycles each per scheduler, 1024 a tile at 64 rows) and 4 times the conversions come to more from 33 rows on.
+// Measured: 16 tokens over 131072 at 32/8/64 (int8) 57.6 us with the merge (2.3 TB/s), against 91 for the other kernel.
 // The order of keys within a page is free as long as P and V agree: V's 16-byte row c of a dim holds the keys 2c, 2c + 1,
 // 2c + 8, 2c + 9, 16 + 2c, 17 + 2c, 24 + 2c, 25 + 2c, which is how a lane finds them in the cache.
 #pragma once
@@ -118,7 +124,19 @@ __global__ __launch_bounds__(kTcThreads, 1) void kv8_attend_tc_kernel(Kv8AttnArg
     const bool row_ok = r < rows, warp_ok = row0 + 16 * quad < rows;
     const int t = r / a.group, qpos = a.ctx_len + t;
     const int row = t * a.q_heads + h * a.group + (r - t * a.group);
-    // Q: the two warpgroups and halves take a quarter of the row's chunks each.
+    // Q: the two warpgroups and halves take a quarter of the row's chunks each. The K tile holds int8 codes with their bias
+    // (decode_raw: one instruction per pair), which comes to a constant per row.
+    float bias = 0.f;
+    if (!E4M3 && row_ok) {
+      const uint4* src = reinterpret_cast<const uint4*>(a.q + t * a.q_stride + (int64_t)(h * a.group + (r - t * a.group)) * D);
+#pragma unroll 4
+      for (int i = 0; i < D / 8; ++i) {
+        const uint4 v = src[i];
+        const float2 s0 = fadd2(unpack_half2(v.x), unpack_half2(v.y)), s1 = fadd2(unpack_half2(v.z), unpack_half2(v.w));
+        bias += (s0.x + s0.y) + (s1.x + s1.y);
+      }
+      bias *= -kCodeBias<E4M3>;
+    }
     {
       const uint4* src = reinterpret_cast<const uint4*>(a.q + t * a.q_stride + (int64_t)(h * a.group + (r - t * a.group)) * D);
 #pragma unroll
@@ -145,7 +163,11 @@ __global__ __launch_bounds__(kTcThreads, 1) void kv8_attend_tc_kernel(Kv8AttnArg
       tc_fence_after();
       const uint32_t s_col = 64 * g;
       if (warp_ok) {
-        const float4 sc0 = sScale[(jt & 7) * 4 + 2 * hh], sc1 = sScale[(jt & 7) * 4 + 2 * hh + 1];
+        float4 sc0 = sScale[(jt & 7) * 4 + 2 * hh], sc1 = sScale[(jt & 7) * 4 + 2 * hh + 1];
+        if (!E4M3) {   // .w: whether the page holds biased codes (an open page does not)
+          sc0.y = fmaf(sc0.w * bias, sc0.x, sc0.y);
+          sc1.y = fmaf(sc1.w * bias, sc1.x, sc1.y);
+        }
         const int k0 = (tile0 + jt) * kTcTile + 64 * hh;
         const bool open = k0 + 63 <= a.ctx_len && (a.window == 0 || k0 > kv_end - 1 - a.window);
         const int lo = (a.window > 0 ? qpos - a.window + 1 : 0) - k0, hi = qpos - k0;
@@ -344,18 +366,18 @@ __global__ __launch_bounds__(kTcThreads, 1) void kv8_attend_tc_kernel(Kv8AttnArg
         ++taken;
         const uint8_t* src = ring + st * raw_bytes;
         if (!is_v) {
-          const float ks = reinterpret_cast<const float*>(src)[0];
+          const float ks = reinterpret_cast<const float*>(src)[0] * kCodeUnit<E4M3>;
           const float vs = reinterpret_cast<const float*>(src)[1];
-          scale = make_float4(ks * a.qk_scale, __log2f(vs), __fdividef(1.f, vs), 0.f);
+          scale = make_float4(ks * a.qk_scale, __log2f(vs), __fdividef(1.f, vs), 1.f);
           const uint4* k4 = reinterpret_cast<const uint4*>(src + S::kOffK);
 #pragma unroll
           for (int s = 0; s < 4 * (D / 64); ++s) {   // 8 keys (s / (D / 64)) x 64 dims
             const uint4 w = k4[s * 32 + g * 4 + c];
             uint4* o = reinterpret_cast<uint4*>(dst + ((s / (D / 64)) * (D / 8) + (s % (D / 64)) * 8 + 2 * c) * 128 + g * 16);
-            o[0] = make_uint4(decode_pair<E4M3, false>(w.x), decode_pair<E4M3, true>(w.x), decode_pair<E4M3, false>(w.y),
-                              decode_pair<E4M3, true>(w.y));
-            o[8] = make_uint4(decode_pair<E4M3, false>(w.z), decode_pair<E4M3, true>(w.z), decode_pair<E4M3, false>(w.w),
-                              decode_pair<E4M3, true>(w.w));
+            o[0] = make_uint4(decode_raw<E4M3, false>(w.x), decode_raw<E4M3, true>(w.x), decode_raw<E4M3, false>(w.y),
+                              decode_raw<E4M3, true>(w.y));
+            o[8] = make_uint4(decode_raw<E4M3, false>(w.z), decode_raw<E4M3, true>(w.z), decode_raw<E4M3, false>(w.w),
+                              decode_raw<E4M3, true>(w.w));
           }
         } else {
           const uint4* v4 = reinterpret_cast<const uint4*>(src);
@@ -399,7 +421,6 @@ __global__ __launch_bounds__(kTcThreads, 1) void kv8_attend_tc_kernel(Kv8AttnArg
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&out_full[buf]);
-      if (aborted()) break;
     }
     if (!ok) atomicExch(&s_abort, 1);
     // Copies still landing after an early exit (bounded).

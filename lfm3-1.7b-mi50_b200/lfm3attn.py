@@ -520,12 +520,14 @@ class LayerCache8:
         self._new, self._like, self._f16, self._f32 = torch.empty, torch.empty_like, torch.float16, torch.float32
 
     def workspace(self, tokens: int, q_heads: int):
-        """A device workspace for verify (up to 32 tokens) and prefill calls of this many tokens at any length."""
+        """A device workspace for verify or prefill calls of up to this many tokens at any length of this cache."""
         import torch
 
-        need = lib().lfm3a_kv8_prefill_workspace_bytes(ctypes.byref(self.layout), tokens, q_heads, self.capacity)
-        if tokens <= 32:   # no staging
-            need = lib().lfm3a_verify_workspace_bytes(tokens, q_heads, self.head_dim, self.splits(q_heads, 1 << 30, tokens))
+        need = max(lib().lfm3a_verify_workspace_bytes(m, q_heads, self.head_dim, self.splits(q_heads, 1 << 30, m))
+                   for m in range(1, min(tokens, 32) + 1))
+        if tokens > 32:
+            need = max(need, lib().lfm3a_kv8_prefill_workspace_bytes(ctypes.byref(self.layout), tokens, q_heads,
+                                                                     self.capacity))
         return torch.empty(need, dtype=torch.uint8, device=self.pool.device)
 
     def splits(self, q_heads: int, ctx_len: int, m: int, window: int = 0) -> int:
