@@ -507,6 +507,8 @@ class LayerCache8:
             self.pool = torch.zeros(self.pool_blocks * self.layout.block_bytes, dtype=torch.uint8, device=device)
         if block_table is None:
             block_table = torch.arange(max(1, logical), dtype=torch.int32, device=device)
+        if block_table.dtype != torch.int32 or block_table.numel() < logical or not block_table.is_contiguous():
+            raise LFM3AError(EINVAL, "block_table must hold an int32 for every 32 tokens of the capacity")
         self.table = block_table
         self.tail = torch.zeros(lib().lfm3a_kv8_tail_bytes(ctypes.byref(self.layout)), dtype=torch.uint8, device=device)
         self.length = self.sealed = 0
@@ -538,10 +540,17 @@ class LayerCache8:
 
     def append(self, k, v, pos0: int | None = None, rope=None, k_norm=None, token_stride: int = 0, draft: bool = False,
                stream=None) -> None:
-        """Stores k, v ([n][kv_heads][head_dim] fp16 device tensors) at positions pos0.. (default: the end). draft: the
-        new tokens may be rolled back, so only tokens below pos0 are sealed."""
+        """Stores k, v ([n][kv_heads][head_dim] fp16 device tensors, tokens strided alike) at positions pos0.. (default:
+        the end). draft: the new tokens may be rolled back, so only tokens below pos0 are sealed."""
         pos0 = self.length if pos0 is None else pos0
-        n = k.shape[0]
+        n, row = k.shape[0], self.kv_heads * self.head_dim
+        if k.dtype != self._f16 or v.dtype != self._f16 or k.shape != v.shape or k.numel() != n * row or not (
+                k.is_cuda and v.is_cuda):
+            raise LFM3AError(EINVAL, "k and v must be fp16 [n][kv_heads][head_dim] on the GPU")
+        if not (k.is_contiguous() and v.is_contiguous()) and n > 0:
+            if not (k[0].is_contiguous() and v[0].is_contiguous()) or k.stride(0) != v.stride(0) and n > 1:
+                raise LFM3AError(EINVAL, "k and v need contiguous rows and one token stride")
+            token_stride = token_stride or max(row, k.stride(0))
         if pos0 + n > self.capacity:
             raise LFM3AError(EINVAL, "append past the cache capacity")
         if pos0 > self.length:
@@ -570,17 +579,31 @@ class LayerCache8:
     def _check_q(self, q, ctx_len: int) -> tuple[int, int, int]:
         m, qh, d = q.shape
         st, sh, sd = q.stride()
-        if d != self.head_dim or sd != 1 or (qh > 1 and sh != d):
-            raise LFM3AError(EINVAL, "q must be [tokens][q_heads][head_dim] with contiguous rows")
+        if q.dtype != self._f16 or not q.is_cuda or d != self.head_dim or sd != 1 or (qh > 1 and sh != d):
+            raise LFM3AError(EINVAL, "q must be fp16 [tokens][q_heads][head_dim] on the GPU with contiguous rows")
         if ctx_len < 0 or ctx_len + m > self.length:
             raise LFM3AError(EINVAL, "the queries' tokens must be appended first")
         return m, qh, st if m > 1 else qh * d
+
+    def _check_f16(self, shape, t) -> None:
+        if t.dtype != self._f16 or t.shape != shape or not t.is_contiguous() or not t.is_cuda:
+            raise LFM3AError(EINVAL, "gate [m][q_heads] and out (q's shape) must be contiguous fp16 on the GPU")
+
+    def _check_lse(self, lse, m: int, qh: int) -> None:
+        if lse.dtype != self._f32 or lse.shape != (m, qh) or not lse.is_contiguous() or not lse.is_cuda:
+            raise LFM3AError(EINVAL, "lse must be fp32 [m][q_heads] on the GPU")
 
     def verify(self, q, ctx_len: int, window: int = 0, gate=None, out=None, lse=None, workspace=None, splits: int = 0,
                stream=None):
         """Attention of q ([m][q_heads][head_dim] fp16, row-strided) at ctx_len.., m <= 32; the tokens' K/V appended.
         lse: fp32 [m][q_heads] to fill with each row's log-sum-exp. Returns fp16 [m][q_heads][head_dim]."""
         m, qh, stride = self._check_q(q, ctx_len)
+        if gate is not None:
+            self._check_f16((m, qh), gate)
+        if out is not None:
+            self._check_f16(q.shape, out)
+        if lse is not None:
+            self._check_lse(lse, m, qh)
         if out is None:
             out = self._like(q) if q.is_contiguous() else self._new(q.shape, dtype=self._f16, device=q.device)
         if workspace is None:
@@ -602,7 +625,9 @@ class LayerCache8:
         import torch
 
         t, qh, stride = self._check_q(q, context)
-        if out is None:
+        if out is not None:
+            self._check_f16(q.shape, out)
+        else:
             out = torch.empty((t, qh, self.head_dim), dtype=torch.float16, device=q.device)
         if t == 0:
             return out
@@ -618,14 +643,14 @@ class LayerCache8:
         """fp32 [kv_heads][ctx_len + m]: decay * prev plus the attention weight each key got from the m tokens of q,
         summed over the query heads of its kv head. lse: of verify for the same q."""
         m, qh, stride = self._check_q(q, ctx_len)
-        if lse.dtype != self._f32 or tuple(lse.shape) != (m, qh) or not lse.is_contiguous():
-            raise LFM3AError(EINVAL, "lse must be fp32 [m][q_heads]")
+        self._check_lse(lse, m, qh)
         n = ctx_len + m
         if out is None:
             out = self._new((self.kv_heads, n), dtype=self._f32, device=q.device)
         for t in (out, prev):
-            if t is not None and (t.dtype != self._f32 or t.shape[0] != self.kv_heads or t.stride(1) != 1):
-                raise LFM3AError(EINVAL, "weights must be fp32 [kv_heads][>= ctx_len + m]")
+            if t is not None and (t.dtype != self._f32 or t.shape[0] != self.kv_heads or t.shape[1] < n or t.stride(1) != 1
+                                  or not t.is_cuda):
+                raise LFM3AError(EINVAL, "weights must be fp32 [kv_heads][>= ctx_len + m] on the GPU")
         _check(self._weights(self._view, q.data_ptr(), stride, m, qh, ctx_len, self.sealed_below(n), window,
                              lse.data_ptr(), _ptr(prev), 0 if prev is None else prev.stride(0), decay, out.data_ptr(),
                              out.stride(0), _stream(stream)))
@@ -637,6 +662,8 @@ class LayerCache8:
         (keep int32 [kv_heads][budget], the kept keys' weights)."""
         if dst is self or budget > dst.capacity:
             raise LFM3AError(EINVAL, "eviction needs another cache with room for the budget")
+        if weights.shape[0] != self.kv_heads or dst.mode != self.mode or dst.layout.block_bytes != self.layout.block_bytes:
+            raise LFM3AError(EINVAL, "eviction needs weights of each kv head and a cache of the same layout")
         keep, kept = evict_select(weights, self.length, budget, sink, recent, stream=stream)
         _check(self._compact(self._view, self.length, self.sealed, keep.data_ptr(), budget, dst._view, _stream(stream)))
         dst.length, dst.sealed = budget, budget // BLOCK_TOKENS * BLOCK_TOKENS
@@ -649,8 +676,8 @@ def evict_select(weights, length: int, budget: int, sink: int, recent: int, stre
 
     h, width = weights.shape
     row, one = weights.stride()
-    if weights.dtype != torch.float32 or width < length or one != 1:
-        raise LFM3AError(EINVAL, "weights must be fp32 [kv_heads][>= length]")
+    if weights.dtype != torch.float32 or width < length or one != 1 or not weights.is_cuda:
+        raise LFM3AError(EINVAL, "weights must be fp32 [kv_heads][>= length] on the GPU")
     kept = weights.new_empty((h, max(0, budget)))
     keep = torch.empty_like(kept, dtype=torch.int32)
     _check(lib().lfm3a_evict_select(weights.data_ptr(), row, h, length, sink, recent, budget, keep.data_ptr(),
