@@ -1,8 +1,6 @@
 // Eviction from the 8-bit cache by accumulated attention weight: which keys of each kv head stay (evict_select_kernel)
 // and their move into a smaller cache (kv8_compact_kernel).
 #pragma once
-#include <cooperative_groups.h>
-
 #include "kv8.cuh"
 
 namespace lfm3a {
@@ -38,7 +36,6 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 // 8.0 us, 8 x 1000 4.9 us.
 template <int C>
 __device__ __forceinline__ void evict_select(const EvictArgs& a) {
-  namespace cg = cooperative_groups;
   constexpr int W = kEvictThreads / 32;
   __shared__ __align__(16) uint32_t hist[4][256];
   __shared__ uint32_t found[4][2];     // per pass: the digit, and how many keys lie above it

@@ -1232,6 +1232,14 @@ int kv8_splits_for(int kv_heads, int head_dim, int rows, int pages, int sm_count
   return std::min(std::min(splits, std::max(1, (pages + least - 1) / least)), kKv8MaxSplits);
 }
 
+// A kv head's pages that would make 2 to kKv8Cluster splits of one page a warp go to one cluster instead, which merges
+// without a second launch, where all clusters run at once.
+bool kv8_one_cluster(int kv_heads, int head_dim, int rows, int pages, int splits, int sm_count) {
+  const int nr = kv8_rows_per_block(rows), groups = kv_heads * ((rows + nr - 1) / nr);
+  return nr < 64 && splits > 1 && pages <= kKv8Cluster * (head_dim == 64 ? 8 : 12) &&
+         groups * kKv8Cluster <= (head_dim == 64 ? 2 : 1) * sm_count;
+}
+
 int kv8_pages(int ctx_len, int m, int window, int* begin) {
   const int start = window > 0 ? std::max(0, ctx_len - window + 1) : 0;
   *begin = start / kBlockTokens;
@@ -1360,37 +1368,45 @@ int lfm3a_kv8_attention(const lfm3a_kv8_view* kv, const void* q, int64_t q_strid
   a.p_total = kv8_pages(ctx_len, m, window, &a.p_begin);
   a.qk_scale = (1.f / sqrtf((float)D)) * kLog2e;
   const int rows = m * group;
-  if (splits <= 0) splits = kv8_splits_for(H, D, rows, a.p_total, current_sm_count());
+  const int nr = kv8_rows_per_block(rows), groups = (rows + nr - 1) / nr;
+  bool cluster = false;
+  if (splits <= 0) {
+    splits = kv8_splits_for(H, D, rows, a.p_total, current_sm_count());
+    cluster = kv8_one_cluster(H, D, rows, a.p_total, splits, current_sm_count());
+  }
   // No split without a page (or a tile of four).
   const int units = kv8_rows_per_block(rows) < 64 ? a.p_total : (a.p_begin + a.p_total - 1) / 4 - a.p_begin / 4 + 1;
   a.splits = std::min(std::min(splits, units), kKv8MaxSplits);
   a.part = nullptr;
-  if (a.splits > 1) {
+  if (cluster) a.splits = kKv8Cluster;
+  if (a.splits > 1 && !cluster) {
     if (!workspace || !aligned16(workspace)) return fail(LFM3A_EINVAL, "kv8 attention needs a 16-byte aligned workspace");
     if (workspace_bytes < lfm3a_verify_workspace_bytes(m, q_heads, D, a.splits))
       return fail(LFM3A_EWORKSPACE, "kv8 attention workspace too small");
     a.part = static_cast<float*>(workspace);
   }
   const cudaStream_t st = as_stream(stream);
-  static std::atomic<bool> done[12][64];
-  const int nr = kv8_rows_per_block(rows);
-  const dim3 grid(a.splits, H, (rows + nr - 1) / nr);
+  static std::atomic<bool> done[20][64];
+  const dim3 grid(a.splits, H, groups);
   rc = with_format(L, [&](auto d, auto f) {
     constexpr int DD = decltype(d)::value;
     constexpr bool E = decltype(f)::value;
-    constexpr int slot = (DD == 64 ? 0 : 6) + (E ? 3 : 0);
+    constexpr int slot = (DD == 64 ? 0 : 10) + (E ? 5 : 0);
     auto run = [&](auto kernel, int smem, int threads, int i) {
       const int r = ensure_smem(kernel, smem, done[slot + i]);
       if (r == LFM3A_OK) launch_pdl(kernel, grid, threads, smem, st, a);
       return r;
     };
+    if (cluster && nr == 8)
+      return run(kv8_attend_cluster_kernel<DD, 1, E>, Kv8Attn<DD, 1>::kSmem, Kv8Attn<DD, 1>::kThreads, 3);
+    if (cluster) return run(kv8_attend_cluster_kernel<DD, 2, E>, Kv8Attn<DD, 2>::kSmem, Kv8Attn<DD, 2>::kThreads, 4);
     if (nr == 8) return run(kv8_attend_kernel<DD, 1, E>, Kv8Attn<DD, 1>::kSmem, Kv8Attn<DD, 1>::kThreads, 0);
     if (nr == 16) return run(kv8_attend_kernel<DD, 2, E>, Kv8Attn<DD, 2>::kSmem, Kv8Attn<DD, 2>::kThreads, 1);
     return run(kv8_attend_tc_kernel<DD, E>, Kv8Tc<DD>::kSmem, kTcThreads, 2);
   });
   if (rc != LFM3A_OK) return rc;
   rc = check_launch("kv8_attend_kernel");
-  if (rc != LFM3A_OK || a.splits == 1) return rc;
+  if (rc != LFM3A_OK || a.splits == 1 || cluster) return rc;
   if (D == 64) launch_pdl(kv8_combine_kernel<64>, m * q_heads, 128, 0, st, a.part, a.splits, a.gate, a.out, lse);
   else launch_pdl(kv8_combine_kernel<128>, m * q_heads, 256, 0, st, a.part, a.splits, a.gate, a.out, lse);
   return check_launch("kv8_combine_kernel");
