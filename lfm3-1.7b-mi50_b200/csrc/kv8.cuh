@@ -552,25 +552,32 @@ __device__ __forceinline__ uint32_t tail_v_pair(const TailView& t, int key, int 
   return w;
 }
 
-// -kCodeBias times the sum of each query row's values, by whole warps (order fixed).
+// -kCodeBias times the sum of each query row's values, a row by D / 8 lanes (order fixed). The loads of several rows go out
+// together: one row after the other they took 5 us of the weights of 128 rows.
 template <int D>
 __device__ __forceinline__ void stage_bias(const __half* q, int64_t q_stride, int rows, int group, int h, int row0, int count,
                                            float bias, float* dst, int warp, int warps, int lane) {
-  for (int i = warp; i < count; i += warps) {
-    const int r = row0 + i;
-    float sum = 0.f;
-    if (r < rows) {
-      const int t = r / group, j = r - t * group;
-      const __half* src = q + t * q_stride + (int64_t)(h * group + j) * D;
+  constexpr int R = D / 8, P = 32 / R, U = 4;
+  for (int i0 = warp * P + lane / R; i0 - lane / R < count; i0 += U * warps * P) {
+    uint4 v[U];
 #pragma unroll
-      for (int k = 0; k < D / 64; ++k) {
-        const float2 f = unpack_half2(reinterpret_cast<const uint32_t*>(src)[lane + 32 * k]);
-        sum += f.x + f.y;
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * warps * P, r = row0 + i;
+      v[u] = make_uint4(0, 0, 0, 0);
+      if (i < count && r < rows) {
+        const int t = r / group, j = r - t * group;
+        v[u] = reinterpret_cast<const uint4*>(q + t * q_stride + (int64_t)(h * group + j) * D)[lane % R];
       }
     }
 #pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) dst[i] = -bias * sum;
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * warps * P;
+      const float2 a = fadd2(unpack_half2(v[u].x), unpack_half2(v[u].y)), b = fadd2(unpack_half2(v[u].z), unpack_half2(v[u].w));
+      float sum = (a.x + a.y) + (b.x + b.y);
+#pragma unroll
+      for (int o = R / 2; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (lane % R == 0 && i < count) dst[i] = -bias * sum;
+    }
   }
 }
 
@@ -1210,7 +1217,8 @@ struct Kv8Weights {
   static __host__ __device__ constexpr int lse_off(int ntiles) { return kRing + ntiles * 8 * D * 2; }
   static __host__ __device__ constexpr int bias_off(int ntiles) { return lse_off(ntiles) + ntiles * 8 * 4; }
   static __host__ __device__ constexpr int bar_off(int ntiles) { return bias_off(ntiles) + ntiles * 8 * 4; }
-  static __host__ __device__ constexpr int smem(int ntiles) { return bar_off(ntiles) + kWarps * kStages * 8; }
+  static __host__ __device__ constexpr int part_off(int ntiles) { return bar_off(ntiles) + kWarps * kStages * 8; }
+  static __host__ __device__ constexpr int smem(int ntiles) { return part_off(ntiles) + kThreads * 4; }
 };
 
 // out[h][key] = decay prev[h][key] + sum over the m tokens and the head's query rows of 2^(s - lse): only K is read. A
@@ -1218,9 +1226,11 @@ struct Kv8Weights {
 // independent chains of MMAs (16 keys each) per 8 rows; a lane owns the weights of 4 keys for 2 rows in 8, so the sums
 // meet in two shuffles per page and no atomics are needed. prev is loaded a page ahead (loaded when wanted, its latency
 // was two thirds of the time of a single token's pass). Grid (splits, kv heads). Bound by HBM and the latency of a page's
-// chain of MMAs for one token (131072 tokens at 32/8/64: 19.2 us, 3.9 TB/s), by the MMAs and the uneven last round of
-// pages for many rows (32 tokens over 20000 at 16/4/128: 15.4 us).
-template <int D, bool E4M3>
+// chain of MMAs for one token (131072 tokens at 32/8/64: 19.2 us with a sum so far, 3.9 TB/s), by the MMAs for many rows.
+// SHARE: in a last round with half of a block's warps or less to do, 2 to 8 warps share a page's rows, and their sums meet
+// in shared memory. It costs the loop some instructions: int8, 32/8/64, 32 tokens over 20000 17.0 us against 19.1 without
+// (2 rounds of pages), 4 tokens over 131000 22.8 against 20.5 (16 rounds), so kv8_weights_share picks it for few rounds.
+template <int D, bool E4M3, bool SHARE>
 __global__ __launch_bounds__(Kv8Weights<D>::kThreads, 2) void kv8_weights_kernel(Kv8WeightArgs a) {
   using L = Kv8Weights<D>;
   using S = Q8Section<D>;
@@ -1247,11 +1257,21 @@ __global__ __launch_bounds__(Kv8Weights<D>::kThreads, 2) void kv8_weights_kernel
     mbar_arrive_expect_tx(&full[st], L::kStageBytes);
     bulk_g2s(ring + st * L::kStageBytes, head + phys_block(a.g, page) * a.g.block_bytes, L::kStageBytes, &full[st]);
   };
-  const int first = pg0 + warp;
+  // This warp's pages in order: one of each 8; of a last round with half of the warps or less to do, a share of the rows.
+  const int whole = (pg1 - pg0) / W, rest = (pg1 - pg0) % W;
+  int share = !SHARE || rest == 0 || rest > W / 2 ? 1 : rest == 1 ? 8 : rest == 2 ? 4 : 2;   // warps to a page of the last round
+  if (SHARE)
+    while (share > ntiles) share /= 2;
+  const int last = min(pg1, pg0 + whole * W + warp / share), sub = SHARE ? warp % share : 0;
+  auto page_of = [&](int k) {   // pg1 or more past the last one
+    return !SHARE || k < whole ? pg0 + k * W + warp : k == whole ? last : pg1;
+  };
+  const int end = min(pg1, sealed_pages);
   int issued = 0, waited = 0;
-  if (lane == 0)
-    for (int p = first; issued < NS && p < pg1 && p < sealed_pages; p += W) issue(p, issued++);
-  issued = __shfl_sync(0xffffffffu, issued, 0);
+  while (issued < NS && page_of(issued) < end) {
+    if (lane == 0) issue(page_of(issued), issued);
+    ++issued;
+  }
   stage_q<D>(a.q, a.q_stride, rows, a.group, h, 0, ntiles, sq, threadIdx.x, L::kThreads);
   if (!E4M3) stage_bias<D>(a.q, a.q_stride, rows, a.group, h, 0, 8 * ntiles, kCodeBias<E4M3>, sbias, warp, W, lane);
   for (int r = threadIdx.x; r < 8 * ntiles; r += L::kThreads) {
@@ -1263,11 +1283,12 @@ __global__ __launch_bounds__(Kv8Weights<D>::kThreads, 2) void kv8_weights_kernel
   __syncthreads();
 
   const TailView tail = tail_of(a.tail, a.g.kv_heads, h, D);
-  // The page's 32 keys against all rows; lane i adds key i's sum to old and stores it.
-  auto rows32 = [&](const uint32_t (&f)[2][4 * NE][4], int page, bool open, float kc, float old, bool biased) {
+  float* spart = reinterpret_cast<float*>(smem + L::part_off(ntiles));
+  // The page's 32 keys against all rows, or a share of them; lane i adds key i's sum to old and stores it.
+  auto rows32 = [&](const uint32_t (&f)[2][4 * NE][4], int page, bool shared, bool open, float kc, float old, bool biased) {
     float w[4] = {0.f, 0.f, 0.f, 0.f};   // keys 8 i + g
 #pragma unroll 2
-    for (int n = 0; n < ntiles; ++n) {
+    for (int n = SHARE && shared ? sub : 0; n < ntiles; n += SHARE && shared ? share : 1) {
       float2 bias = make_float2(0.f, 0.f);
       if (!E4M3 && biased) bias = *reinterpret_cast<const float2*>(sbias + 8 * n + 2 * c);
       float s[2][4] = {{bias.x, bias.y, bias.x, bias.y}, {bias.x, bias.y, bias.x, bias.y}};
@@ -1305,18 +1326,20 @@ __global__ __launch_bounds__(Kv8Weights<D>::kThreads, 2) void kv8_weights_kernel
       if ((lane >> 3) == i) mine = v;
     }
     const int key = page * kBlockTokens + lane;
-    if (key < kv_end) a.out[h * a.out_stride + key] = fmaf(a.decay, old, mine);
+    if (SHARE && shared) spart[warp * 32 + lane] = mine;
+    else if (key < kv_end) a.out[h * a.out_stride + key] = fmaf(a.decay, old, mine);
   };
   auto load_prev = [&](int page) -> float {
     const int key = page * kBlockTokens + lane;
     return a.prev && page < pg1 && key < kv_end ? a.prev[h * a.prev_stride + key] : 0.f;
   };
 
-  float old_next = load_prev(first);
+  float old_next = load_prev(page_of(0));
   bool ok = true;
-  int st = 0, next = first + issued * W;
+  int st = 0, k = 0;
   uint32_t phase = 0;
-  for (int page = first; page < pg1 && page < sealed_pages; page += W) {
+  for (; page_of(k) < end; ++k) {
+    const int page = page_of(k);
     ok = __all_sync(0xffffffffu, mbar_wait(&full[st], phase));
     if (!ok) break;
     ++waited;
@@ -1324,7 +1347,7 @@ __global__ __launch_bounds__(Kv8Weights<D>::kThreads, 2) void kv8_weights_kernel
     const float kc = reinterpret_cast<const float*>(sec)[0] * kCodeUnit<E4M3> * a.qk_scale;
     const bool open = page_open(page, a.ctx_len, a.m, a.window);
     const float old = old_next;
-    old_next = load_prev(page + W);
+    old_next = load_prev(page_of(k + 1));
     uint32_t f[2][4 * NE][4];
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt) {
@@ -1342,13 +1365,12 @@ __global__ __launch_bounds__(Kv8Weights<D>::kThreads, 2) void kv8_weights_kernel
         }
       }
     }
-    rows32(f, page, open, kc, old, true);
+    rows32(f, page, SHARE && share > 1 && k == whole, open, kc, old, true);
     __syncwarp();
-    if (next < pg1 && next < sealed_pages) {
-      if (lane == 0) issue(next, st);
+    if (page_of(issued) < end) {
+      if (lane == 0) issue(page_of(issued), st);
       ++issued;
     }
-    next += W;
     if (++st == NS) {
       st = 0;
       phase ^= 1;
@@ -1364,9 +1386,8 @@ __global__ __launch_bounds__(Kv8Weights<D>::kThreads, 2) void kv8_weights_kernel
       }
     }
   }
-  int page = first;
-  if (page < sealed_pages) page += (sealed_pages - page + W - 1) / W * W;
-  for (; page < pg1; page += W) {
+  for (; ok && page_of(k) < pg1; ++k) {
+    const int page = page_of(k);
     uint32_t f[2][4 * NE][4];
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt)
@@ -1382,7 +1403,16 @@ __global__ __launch_bounds__(Kv8Weights<D>::kThreads, 2) void kv8_weights_kernel
           f[mt][4 * e + u][3] = kB[u].y;
         }
       }
-    rows32(f, page, false, a.qk_scale, load_prev(page), false);
+    rows32(f, page, SHARE && share > 1 && k == whole, false, a.qk_scale, load_prev(page), false);
+  }
+  if (SHARE && share > 1) {   // the shares of the last round's pages meet, in the warps' order
+    __syncthreads();
+    const int key = last * kBlockTokens + lane;
+    if (sub == 0 && last < pg1 && key < kv_end) {
+      float sum = 0.f;
+      for (int i = 0; i < share; ++i) sum += spart[(warp + i) * 32 + lane];
+      a.out[h * a.out_stride + key] = fmaf(a.decay, load_prev(last), sum);
+    }
   }
 }
 

@@ -1240,6 +1240,11 @@ bool kv8_one_cluster(int kv_heads, int head_dim, int rows, int pages, int splits
          groups * kKv8Cluster <= (head_dim == 64 ? 2 : 1) * sm_count;
 }
 
+// Whether kv8_weights_kernel's warps share the rows of a last round's pages: 32 rows or more, and at most 5 rounds of pages.
+// At 32/8/64 (int8), with and without: over 20000 (2.1 rounds) 4 tokens 7.5 and 6.8 us, 8 tokens 8.6 and 9.2; over 40000
+// 16 tokens 17.4 and 18.1, 32 tokens 26.7 and 29.7; over 131000 (14 rounds) 8 tokens 29.3 and 27.0.
+bool kv8_weights_share(int ntiles, int pages, int blocks) { return ntiles >= 4 && pages <= 5 * 8 * blocks; }
+
 int kv8_pages(int ctx_len, int m, int window, int* begin) {
   const int start = window > 0 ? std::max(0, ctx_len - window + 1) : 0;
   *begin = start / kBlockTokens;
@@ -1547,19 +1552,23 @@ int lfm3a_kv8_weights(const lfm3a_kv8_view* kv, const void* q, int64_t q_stride,
   a.pages = (len + kBlockTokens - 1) / kBlockTokens;
   a.decay = decay;
   a.qk_scale = (1.f / sqrtf((float)D)) * kLog2e;
-  // Two blocks per SM (up to 128 rows; more rows' operands leave room for one), a page for each of a block's 8 warps.
-  a.splits = std::max(1, std::min(2 * current_sm_count() / H, (a.pages + 7) / 8));
-  const int ntiles = (m * group + 7) / 8;
+  // Two blocks per SM (up to 128 rows; more rows' operands leave room for one), a page for each of a block's 8 warps, or
+  // for two of them where they share its rows.
+  const int ntiles = (m * group + 7) / 8, most = std::max(1, 2 * current_sm_count() / H);
+  const bool share = kv8_weights_share(ntiles, a.pages, most);
+  a.splits = std::min(most, (a.pages + (share ? 3 : 7)) / (share ? 4 : 8));
   const cudaStream_t st = as_stream(stream);
-  static std::atomic<bool> done[4][64];
+  static std::atomic<bool> done[8][64];
   rc = with_format(L, [&](auto d, auto f) {
     constexpr int DD = decltype(d)::value;
     constexpr bool E = decltype(f)::value;
     using W = Kv8Weights<DD>;
-    const int r = ensure_smem(kv8_weights_kernel<DD, E>, W::smem(W::kMaxRows / 8), done[(DD == 64 ? 0 : 2) + (E ? 1 : 0)]);
-    if (r == LFM3A_OK)
-      launch_pdl(kv8_weights_kernel<DD, E>, dim3(a.splits, H), W::kThreads, W::smem(ntiles), st, a);
-    return r;
+    auto run = [&](auto kernel, int i) {
+      const int r = ensure_smem(kernel, W::smem(W::kMaxRows / 8), done[(DD == 64 ? 0 : 4) + (E ? 2 : 0) + i]);
+      if (r == LFM3A_OK) launch_pdl(kernel, dim3(a.splits, H), W::kThreads, W::smem(ntiles), st, a);
+      return r;
+    };
+    return share ? run(kv8_weights_kernel<DD, E, true>, 1) : run(kv8_weights_kernel<DD, E, false>, 0);
   });
   if (rc != LFM3A_OK) return rc;
   return check_launch("kv8_weights_kernel");

@@ -519,7 +519,7 @@ class LayerCache8:
         handle = lib()
         self._append, self._read, self._attention = handle.lfm3a_kv8_append, handle.lfm3a_kv8_read, handle.lfm3a_kv8_attention
         self._weights, self._compact = handle.lfm3a_kv8_weights, handle.lfm3a_kv8_compact
-        self._new, self._like, self._f16, self._f32 = torch.empty, torch.empty_like, torch.float16, torch.float32
+        self._like, self._f16, self._f32 = torch.empty_like, torch.float16, torch.float32
 
     def workspace(self, tokens: int, q_heads: int):
         """A device workspace for verify or prefill calls of up to this many tokens at any length of this cache."""
@@ -571,7 +571,7 @@ class LayerCache8:
         """(K, V) fp16 [n][kv_heads][head_dim]: the values the cached tokens pos0.. stand for."""
         if pos0 < 0 or n < 0 or pos0 + n > self.length:
             raise LFM3AError(EINVAL, "read past the cached tokens")
-        k = self._new((n, self.kv_heads, self.head_dim), dtype=self._f16, device=self.pool.device)
+        k = self.tail.new_empty((n, self.kv_heads, self.head_dim), dtype=self._f16)
         v = self._like(k)
         _check(self._read(self._view, pos0, n, self.sealed, k.data_ptr(), v.data_ptr(), _stream(stream)))
         return k, v
@@ -605,11 +605,10 @@ class LayerCache8:
         if lse is not None:
             self._check_lse(lse, m, qh)
         if out is None:
-            out = self._like(q) if q.is_contiguous() else self._new(q.shape, dtype=self._f16, device=q.device)
+            out = self._like(q) if q.is_contiguous() else q.new_empty(q.shape)
         if workspace is None:
             s = splits if splits > 0 else self.splits(qh, ctx_len, m, window)
-            workspace = self._new(lib().lfm3a_verify_workspace_bytes(m, qh, self.head_dim, s) // 4, dtype=self._f32,
-                                  device=q.device)
+            workspace = q.new_empty(lib().lfm3a_verify_workspace_bytes(m, qh, self.head_dim, s) // 4, dtype=self._f32)
         _check(self._attention(self._view, q.data_ptr(), stride, m, qh, ctx_len, self.sealed_below(ctx_len + m), window,
                                _ptr(gate), out.data_ptr(), _ptr(lse), workspace.data_ptr(), workspace.nbytes, splits,
                                _stream(stream)))
@@ -646,7 +645,7 @@ class LayerCache8:
         self._check_lse(lse, m, qh)
         n = ctx_len + m
         if out is None:
-            out = self._new((self.kv_heads, n), dtype=self._f32, device=q.device)
+            out = q.new_empty((self.kv_heads, n), dtype=self._f32)
         for t in (out, prev):
             if t is not None and (t.dtype != self._f32 or t.shape[0] != self.kv_heads or t.shape[1] < n or t.stride(1) != 1
                                   or not t.is_cuda):
