@@ -1219,8 +1219,8 @@ int with_format(const lfm3a_kv_layout& L, F f) {
 }
 
 // Query rows of one kv head that a block takes: kv8_attend_kernel's 8 or 16, or the 64 of kv8_attend_tc_kernel. 17 to 32 rows
-// go through the former in two groups: over 131072 tokens at 32/8/64 (int8) 52.7 us against 60.4; 48 rows 72 against 61,
-// 64 rows 91 against 62, 128 rows 191 against 111.
+// go through the former in two groups: over 131072 tokens at 32/8/64 (int8) 51.0 us against 55.7; 48 rows 72 against 57,
+// 64 rows 91 against 58, 128 rows 191 against 105.
 int kv8_rows_per_block(int rows) { return rows <= 8 ? 8 : rows <= 32 ? 16 : 64; }
 
 // Key splits: one wave of resident blocks, at least a page for each of a block's warps (8, 12 at head_dim 128), or a
