@@ -283,6 +283,13 @@ __device__ __forceinline__ float2 ffma2(float2 a, float2 b, float2 c) {
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
   return d;
 }
+// Both values rounded to the 11 significant bits of a normal fp16, in fp32's range: fl(p + 2^13 p) - 2^13 p, each one
+// packed FMA. What pack_half2 makes of the result is exact down to 2^-14. A softmax sum of such P carries the roundings of
+// the fp16 P that the second product reads (where one key dominates they cancel in the quotient), and loses nothing where
+// that P is subnormal or 0.
+__device__ __forceinline__ float2 round11(float2 p) {
+  return ffma2(p, make_float2(-8192.f, -8192.f), ffma2(p, make_float2(8192.f, 8192.f), p));
+}
 __device__ __forceinline__ float2 fadd2(float2 a, float2 b) {
   float2 d;
   asm("{\n\t.reg .b64 ra, rb, rd;\n\t"

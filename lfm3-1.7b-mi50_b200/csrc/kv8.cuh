@@ -713,7 +713,7 @@ __device__ __forceinline__ void kv8_exponents(float (&x)[HB][NT][4], int n, floa
     }
 }
 
-// A warp's running state: O^T accumulators, the maxima of its lanes' rows, the sums of P' / vs, exact and with P' as rounded.
+// A warp's running state: O^T accumulators, the maxima of its lanes' rows, the sums of P' / vs, exact and with P' rounded (round11).
 template <int D, int NT>
 struct Kv8Rows {
   float o[D / 16][NT][4];
@@ -782,10 +782,10 @@ __device__ __forceinline__ void kv8_softmax(const QK& qk, Kv8Rows<D, NT>& w, con
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         const float2 p = make_float2(fast_exp2(x[b][n][2 * k]), fast_exp2(x[b][n][2 * k + 1]));
-        const uint32_t hp = pack_half2(p.x, p.y);
+        const float2 r = round11(p);
         sum = fadd2(sum, p);
-        rsum = fadd2(rsum, unpack_half2(hp));
-        pb[b][n][k] = movmatrix_trans(hp);
+        rsum = fadd2(rsum, r);
+        pb[b][n][k] = movmatrix_trans(pack_half2(r.x, r.y));
       }
     w.l[n] = ffma2(sum, make_float2(inv, inv), w.l[n]);
     w.lp[n] = ffma2(rsum, make_float2(inv, inv), w.lp[n]);
@@ -798,7 +798,8 @@ __device__ __forceinline__ void kv8_softmax(const QK& qk, Kv8Rows<D, NT>& w, con
 // for another before the end, and turns codes into fp16 operands in registers: Q, K and P V products are exact to fp32
 // accumulation, only P is rounded to fp16. Scores come as S^T (keys x rows), so the sealed pages' K scale is one factor
 // per page, and the V scale is folded into the exponent: P' = 2^(s + log2 vs - m'), with m' the running maximum of
-// s + log2 vs, gives sum P' v8 = 2^-m' sum 2^s v directly, and l = sum P' / vs is the softmax sum. m' is lazy (moved
+// s + log2 vs, gives sum P' v8 = 2^-m' sum 2^s v directly, and l = sum P' / vs is the softmax sum, of fp32 P': a page of
+// small vs keeps its share of the sum where its P' is below fp16's normal values (round11). m' is lazy (moved
 // only when a score passes it by 2^8; fp16 P then stays below 2^8 and fp32 sums are unaffected), so the common page
 // needs no shuffles but one vote. movmatrix turns the S^T accumulators into the B operand of O^T = V^T P.
 // The warps meet in shared memory at the end; one split writes its rows, several write (acc, m', l) partials.
@@ -950,7 +951,7 @@ __device__ __forceinline__ void kv8_attend(const Kv8AttnArgs& a) {
       w.l[n] = fadd2(w.l[n], make_float2(__shfl_xor_sync(0xffffffffu, w.l[n].x, x), __shfl_xor_sync(0xffffffffu, w.l[n].y, x)));
       w.lp[n] = fadd2(w.lp[n], make_float2(__shfl_xor_sync(0xffffffffu, w.lp[n].x, x), __shfl_xor_sync(0xffffffffu, w.lp[n].y, x)));
     }
-    // acc / lp is the mean over P' as rounded (numerator and denominator carry the same roundings); from here on acc is
+    // acc / lp is the mean over rounded P' (numerator and denominator carry the same roundings); from here on acc is
     // relative to the exact sum, which the log-sum-exp needs
     const float f[2] = {w.lp[n].x > 0.f ? w.l[n].x / w.lp[n].x : 1.f, w.lp[n].y > 0.f ? w.l[n].y / w.lp[n].y : 1.f};
 #pragma unroll

@@ -230,9 +230,10 @@ __global__ __launch_bounds__(kTcThreads, 1) void kv8_attend_tc_kernel(Kv8AttnArg
               const int k = 8 * i + 2 * c;
               const float2 e = ffma2(make_float2(x[k], x[k + 1]), kf, off);
               const float2 pr = make_float2(fast_exp2(e.x), fast_exp2(e.y));
+              const float2 rr = round11(pr);
               ls = fadd2(ls, pr);
-              w[i] = pack_half2(pr.x, pr.y);
-              lps = fadd2(lps, unpack_half2(w[i]));
+              w[i] = pack_half2(rr.x, rr.y);
+              lps = fadd2(lps, rr);
             }
             *reinterpret_cast<uint4*>(pb + (4 * p + c) * 128) = make_uint4(w[0], w[1], w[2], w[3]);
           }
@@ -260,7 +261,7 @@ __global__ __launch_bounds__(kTcThreads, 1) void kv8_attend_tc_kernel(Kv8AttnArg
     if (g == 0 && done && warp_ok && !aborted()) {
       tc_fence_after();
       const float4 b = sML[32 * quad + lane];
-      // acc / lp is the mean over P as rounded; relative to the exact sums from here on
+      // acc / lp is the mean over rounded P (round11); relative to the exact sums from here on
       const float n0 = lp_run > 0.f ? l_run / lp_run : 1.f, n1 = b.z > 0.f ? b.y / b.z : 1.f;
       float M = fmaxf(m_run, b.x);
       M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, 16));

@@ -274,7 +274,7 @@ struct PfLayout {
 // the plain instantiation reads Q as it is and stores the output ungated.
 // SCALED (exact only): the pool's K and V are 8-bit codes as fp16 with one factor per page and head (kv8.cuh): the K
 // factor multiplies the page's scores, the V factor goes into their exponents (P' = 2^(s + log2 f - m)), whose sum is
-// taken over P' / f, after its rounding to fp16, so that numerator and denominator carry the same roundings.
+// taken over P' / f with P' rounded in fp32 (round11): the numerator's roundings, without fp16's lower end.
 template <int D, bool I8, bool SPLIT, bool GLUE, bool SCALED = false>
 __global__ __launch_bounds__(PfLayout<D, I8>::kThreads, PfLayout<D, I8>::kBlocksPerSm) void prefill_kernel(PrefillArgs a) {
   using L = PfLayout<D, I8>;
@@ -472,8 +472,9 @@ __global__ __launch_bounds__(PfLayout<D, I8>::kThreads, PfLayout<D, I8>::kBlocks
         for (int k = 0; k < 64; k += 2) {
           const int i = k >> 5;
           const float2 g = ffma2(make_float2(x[k], x[k + 1]), make_float2(kf[i], kf[i]), make_float2(vl[i] + neg, vl[i] + neg));
-          pw[k / 2] = pack_half2(fast_exp2(g.x), fast_exp2(g.y));
-          ls[i][(k >> 1) & 1] = fadd2(ls[i][(k >> 1) & 1], unpack_half2(pw[k / 2]));
+          const float2 p = round11(make_float2(fast_exp2(g.x), fast_exp2(g.y)));
+          ls[i][(k >> 1) & 1] = fadd2(ls[i][(k >> 1) & 1], p);
+          pw[k / 2] = pack_half2(p.x, p.y);
         }
         const float2 l0 = fadd2(ls[0][0], ls[0][1]), l1 = fadd2(ls[1][0], ls[1][1]);
         l_run = fmaf(l0.x + l0.y, vr[0], fmaf(l1.x + l1.y, vr[1], l_run));
