@@ -15,6 +15,9 @@ constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kBlockTokens = 32;   // KV block (engine.go:31)
 constexpr int kQuantBlock = 64;    // int8 V block and prefill key tile
 constexpr float kLazy = 8.f;       // prefill_attn.hip:33: rescale only when a tile beats the max by 2^8
+// P of the 8-bit block cache holds its page's V scale and ends as fp16 (2^-14 to 2^16 normal): the running maximum is put
+// 2^7 below the largest P, which with kLazy then stays within 2^15, so P has its 11 bits 2^21 below the largest.
+constexpr float kHeadroom = 7.f;
 
 // Error word raised by a kernel that gives up a bounded wait; the host reads and clears it in
 // lfm3a_sync. A module-scope variable, so kernels reach it without an argument.
@@ -283,13 +286,6 @@ __device__ __forceinline__ float2 ffma2(float2 a, float2 b, float2 c) {
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
   return d;
 }
-// Both values rounded to the 11 significant bits of a normal fp16, in fp32's range: fl(p + 2^13 p) - 2^13 p, each one
-// packed FMA. What pack_half2 makes of the result is exact down to 2^-14. A softmax sum of such P carries the roundings of
-// the fp16 P that the second product reads (where one key dominates they cancel in the quotient), and loses nothing where
-// that P is subnormal or 0.
-__device__ __forceinline__ float2 round11(float2 p) {
-  return ffma2(p, make_float2(-8192.f, -8192.f), ffma2(p, make_float2(8192.f, 8192.f), p));
-}
 __device__ __forceinline__ float2 fadd2(float2 a, float2 b) {
   float2 d;
   asm("{\n\t.reg .b64 ra, rb, rd;\n\t"
@@ -307,6 +303,14 @@ __device__ __forceinline__ float2 fmul2(float2 a, float2 b) {
       : "=f"(d.x), "=f"(d.y)
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return d;
+}
+// Both values rounded to the 11 significant bits of a normal fp16, to nearest even, in fp32's range, by Dekker's split: with
+// c = fl(8193 p), fl(c + fl(p - c)). What pack_half2 makes of the result is exact down to 2^-14. A softmax sum of such P
+// carries the roundings of the fp16 P that the second product reads (where one key dominates they cancel in the quotient),
+// and loses nothing where that P is subnormal or 0.
+__device__ __forceinline__ float2 round11(float2 p) {
+  const float2 c = fmul2(p, make_float2(8193.f, 8193.f));
+  return fadd2(c, ffma2(c, make_float2(-1.f, -1.f), p));
 }
 
 // Launches through a cubin loaded with the CUDA driver API (module.cuh): true when the current device has one and

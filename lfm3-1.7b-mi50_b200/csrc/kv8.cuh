@@ -7,7 +7,8 @@
 // The last tokens (an incomplete page, drafts that may be rolled back) stay in fp16 in a ring of 128 tokens per layer,
 // the tail, so a sealed page depends on committed tokens alone and a rollback needs no device work.
 //
-// Section of one (page, kv head), 32 + 64 D bytes: f32 K scale, f32 V scale, 24 zero bytes, K (32 D bytes), V (32 D).
+// Section of one (page, kv head), 32 + 64 D bytes: f32 K scale, f32 V scale, 4 zero bytes, f32 V factor of the attention
+// kernels' P (the V scale, but 2^-40 for a block of zeros), 16 zero bytes, K (32 D bytes), V (32 D).
 // K and V lie in the order in which the lanes of a warp (g = lane / 4, c = lane % 4) take them as the A operands of
 // mma.m16n8k16: S^T = K Q^T over 16 keys x 8 query rows, and O^T = V^T P over 16 dims x 8 rows. A dot over dims does
 // not care which dim sits at which k, so a lane takes 16 contiguous dims of a key in one 16-byte load:
@@ -29,6 +30,10 @@ namespace lfm3a {
 namespace cg = cooperative_groups;
 
 constexpr int kTailTokens = 128;   // tokens of the fp16 tail ring (slot = position mod 128)
+// V factor of a block of zeros: any serves, its codes being zeros, but a factor above its neighbours' scales would raise
+// the running maximum and push their P out of fp16 (with 1 beside V of 1e-4, e4m3, outputs are off by 0.008 of the RMS).
+constexpr float kZeroFactor = 0x1p-40f;
+constexpr int kFactorWord = 3;     // its place in a section
 
 template <int D>
 struct Q8Section {
@@ -146,8 +151,8 @@ __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
 // ---------------------------------------------------------------- append and sealing
 // A page and kv head is sealed by 2 D threads: the first half of them makes K's codes, the other V's, 16 at a time, two
 // times each. Each gives the largest magnitude of the K and of the V values it has seen and gets the scale of its half
-// and the rounded reciprocal; the header (both scales, zeros) is written. The barrier inside also publishes shared memory
-// written before.
+// and the rounded reciprocal; the header (both scales, the V factor, zeros) is written. The barrier inside also publishes
+// shared memory written before.
 template <int D>
 constexpr int kSealThreads = 2 * D;
 template <int D, bool E4M3>
@@ -170,7 +175,10 @@ __device__ __forceinline__ float2 seal_scale(float kmax, float vmax, float* red,
 #pragma unroll
   for (int i = 0; i < W / 4; ++i) amax = fmaxf(amax, fmaxf(fmaxf(r[i].x, r[i].y), fmaxf(r[i].z, r[i].w)));
   const float scale = amax > 0.f ? __fdiv_rn(amax, E4M3 ? 448.f : 127.f) : 1.f;
-  if (lane < 4 && (warp == 0 || warp == W / 2)) reinterpret_cast<float*>(sec)[2 * lane + is_v] = lane ? 0.f : scale;
+  if (lane < 4 && (warp == 0 || warp == W / 2)) {
+    const int word = 2 * lane + is_v;
+    reinterpret_cast<float*>(sec)[word] = lane == 0 ? scale : word == kFactorWord ? (amax > 0.f ? scale : kZeroFactor) : 0.f;
+  }
   return make_float2(scale, __fdiv_rn(1.f, scale));
 }
 
@@ -722,7 +730,7 @@ struct Kv8Rows {
 };
 
 // Softmax of HB x 16 keys from key0 on, P' packed as B operands. qk(x) makes the scores S^T; kc: their factor, lv: log2 of
-// the V scale, inv: its reciprocal. The scores become exponents in place; the rare page that moves a maximum makes them
+// the V factor, inv: its reciprocal. The scores become exponents in place; the rare page that moves a maximum makes them
 // again (keeping both spills at 16 rows and head_dim 64).
 template <int D, int NT, int HB, typename QK>
 __device__ __forceinline__ void kv8_softmax(const QK& qk, Kv8Rows<D, NT>& w, const Kv8AttnArgs& a, int row, int key0, bool open,
@@ -740,7 +748,7 @@ __device__ __forceinline__ void kv8_softmax(const QK& qk, Kv8Rows<D, NT>& w, con
 #pragma unroll
     for (int b = 0; b < HB; ++b) top = fmax3(fmax3(top, x[b][n][0], x[b][n][1]), x[b][n][2], x[b][n][3]);
   }
-  if (__any_sync(0xffffffffu, top > kLazy)) {
+  if (__any_sync(0xffffffffu, top > kLazy + kHeadroom)) {
     qk.again()(x);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -750,12 +758,13 @@ __device__ __forceinline__ void kv8_softmax(const QK& qk, Kv8Rows<D, NT>& w, con
       float f[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        float mx = w.m[n][i];
+        float mx = -INFINITY;
 #pragma unroll
         for (int b = 0; b < HB; ++b) mx = fmax3(mx, x[b][n][i], x[b][n][i + 2]);
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+        mx = fmaxf(mx - kHeadroom, w.m[n][i]);
         f[i] = mx == -INFINITY ? 1.f : fast_exp2(w.m[n][i] - mx);   // no key yet: 2^-inf = 0
         w.m[n][i] = mx;
         const float m = mx == -INFINITY ? 0.f : mx;
@@ -798,10 +807,10 @@ __device__ __forceinline__ void kv8_softmax(const QK& qk, Kv8Rows<D, NT>& w, con
 // for another before the end, and turns codes into fp16 operands in registers: Q, K and P V products are exact to fp32
 // accumulation, only P is rounded to fp16. Scores come as S^T (keys x rows), so the sealed pages' K scale is one factor
 // per page, and the V scale is folded into the exponent: P' = 2^(s + log2 vs - m'), with m' the running maximum of
-// s + log2 vs, gives sum P' v8 = 2^-m' sum 2^s v directly, and l = sum P' / vs is the softmax sum, of fp32 P': a page of
-// small vs keeps its share of the sum where its P' is below fp16's normal values (round11). m' is lazy (moved
-// only when a score passes it by 2^8; fp16 P then stays below 2^8 and fp32 sums are unaffected), so the common page
-// needs no shuffles but one vote. movmatrix turns the S^T accumulators into the B operand of O^T = V^T P.
+// s + log2 vs less kHeadroom, gives sum P' v8 = 2^-m' sum 2^s v directly, and l = sum P' / vs is the softmax sum, of fp32
+// P': a page of small vs keeps its share of the sum where its P' is below fp16's normal values (round11). m' is lazy (moved
+// only when a score passes it by 2^15; fp16 P then stays within 2^15 and fp32 sums are unaffected), so the common page
+// needs no shuffles but one vote. Open pages come last: their factor of 1 moves m' when the others' P' is summed already. movmatrix turns the S^T accumulators into the B operand of O^T = V^T P.
 // The warps meet in shared memory at the end; one split writes its rows, several write (acc, m', l) partials.
 //
 // What bounds it: HBM for one token (100003 tokens at 32/8/64, int8: 21.6 us with the merge, 4.8 TB/s; 131072: 26.6 us),
@@ -884,7 +893,7 @@ __device__ __forceinline__ void kv8_attend(const Kv8AttnArgs& a) {
     const int page = first + waited * W;
     ++waited;
     const uint8_t* sec = ring + st * L::kStageBytes;
-    const float vs = reinterpret_cast<const float*>(sec)[1];
+    const float vs = reinterpret_cast<const float*>(sec)[kFactorWord];
     const float kc = reinterpret_cast<const float*>(sec)[0] * kCodeUnit<E4M3> * a.qk_scale, lv = __log2f(vs), inv = __fdividef(1.f, vs);
     const bool open = page_open(page, a.ctx_len, a.m, a.window);
     const Kv8Scores<D, NT, HB, E4M3> qk{sec + S::kOffK, sq, sbias, lane};
@@ -1151,7 +1160,7 @@ __global__ __launch_bounds__(128) void kv8_expand_kernel(Kv8ExpandArgs a) {
     const char* sec = a.g.pool + phys_block(a.g, page) * a.g.block_bytes + h * a.g.head_bytes;
     if (tid == 0) {
       const float ks = reinterpret_cast<const float*>(sec)[0];
-      const float vs = reinterpret_cast<const float*>(sec)[1];
+      const float vs = reinterpret_cast<const float*>(sec)[kFactorWord];
       a.scales[section] = make_float4(ks, log2f(vs), 1.f / vs, 0.f);
     }
     // Tile rows of 16 bytes: 8 dims of one key (K), 8 keys of one dim (V).

@@ -198,10 +198,10 @@ __global__ __launch_bounds__(kTcThreads, 1) void kv8_attend_tc_kernel(Kv8AttnArg
           break;
         }
         tc_fence_after();
-        const bool grow = mx > m_run + kLazy;
+        const bool grow = mx > m_run + (kLazy + kHeadroom);
         if (__any_sync(0xffffffffu, grow)) {
-          const float corr = grow ? fast_exp2(m_run - mx) : 1.f;
-          if (grow) m_run = mx;
+          const float corr = grow ? fast_exp2(m_run - (mx - kHeadroom)) : 1.f;
+          if (grow) m_run = mx - kHeadroom;
           l_run *= corr;
           lp_run *= corr;
           if (jt >= 2) {
@@ -368,7 +368,7 @@ __global__ __launch_bounds__(kTcThreads, 1) void kv8_attend_tc_kernel(Kv8AttnArg
         const uint8_t* src = ring + st * raw_bytes;
         if (!is_v) {
           const float ks = reinterpret_cast<const float*>(src)[0] * kCodeUnit<E4M3>;
-          const float vs = reinterpret_cast<const float*>(src)[1];
+          const float vs = reinterpret_cast<const float*>(src)[kFactorWord];
           scale = make_float4(ks * a.qk_scale, __log2f(vs), __fdividef(1.f, vs), 1.f);
           const uint4* k4 = reinterpret_cast<const uint4*>(src + S::kOffK);
 #pragma unroll

@@ -385,6 +385,7 @@ __global__ __launch_bounds__(PfLayout<D, I8>::kThreads, PfLayout<D, I8>::kBlocks
     }
     const uint32_t lane_base = tmem + ((uint32_t)(32 * warp) << 16);
     float m_run = -INFINITY, l_run = 0.f;
+    constexpr float kHead = SCALED ? kHeadroom : 0.f;   // m_run is this far below the running maximum
     // Every wait result is made warp-uniform: the tcgen05.ld/st that follow are warp-collective.
     bool ok = true;
     // The factors of the tile's two pages, loaded a tile ahead (a page past the keys: the first page's).
@@ -436,11 +437,11 @@ __global__ __launch_bounds__(PfLayout<D, I8>::kThreads, PfLayout<D, I8>::kBlocks
       float mx;
       if constexpr (SCALED) mx = fmaxf(fmaf(max32(x), kf[0], vl[0]), fmaf(max32(x + 32), kf[1], vl[1]));
       else mx = max64(x) * a.qk_scale;
-      const bool grow_max = mx > m_run + kLazy;
+      const bool grow_max = mx > m_run + (kLazy + kHead);
       // O lives in TMEM: rescaling it needs the previous PV finished; rare after the first tiles.
       if (__any_sync(0xffffffffu, grow_max)) {
-        const float corr = grow_max ? fast_exp2(m_run - mx) : 1.f;
-        if (grow_max) m_run = mx;
+        const float corr = grow_max ? fast_exp2(m_run - (mx - kHead)) : 1.f;
+        if (grow_max) m_run = mx - kHead;
         l_run *= corr;
         if (jt >= 1) {
           if (!__all_sync(0xffffffffu, mbar_wait(&pv_done[(jt - 1) & 1], (uint32_t)((jt - 1) >> 1) & 1u))) {

@@ -9,7 +9,7 @@ deviations of which stay below the same bound."""
 import numpy as np
 import pytest
 
-from test_gpu_kv8 import BLOCK, FMTS, TOL, attention64, build, dev, rel_err, rows_of, values
+from test_gpu_kv8 import BLOCK, FMTS, TOL, TOL_LSE, attention64, build, dev, rel_err, rows_of, values
 
 pytestmark = pytest.mark.gpu
 
@@ -64,3 +64,75 @@ def test_prefill(la, synth, cuda, fmt, kind, qh, kvh, d, ctx, t, window):
     sealed = n // BLOCK * BLOCK
     want, _ = attention64(q, values(K, sealed, fmt), values(V, sealed, fmt), ctx, window)
     assert rel_err(got.cpu().numpy(), want) < TOL
+
+
+# ------------------------------------------------------------------ pages that must not drown the others' P
+# A block of zeros has a scale of 1 and the open pages are fp16: next to small V neither may push the other pages' P to
+# fp16's lower end, nor may a block whose large V nobody attends to. The tolerance is the one above: P has its 11 bits for
+# keys down to 2^-21 of the largest product, and what is smaller is off by 2^-32 of that product.
+def small(synth, kind, n, m, qh, kvh, d):
+    K, V = (x.astype(np.float32) for x in rows_of(synth, 500 + n, n, kvh, d))
+    q = synth.Stream(600 + n).normal_f16((m, qh, d)).astype(np.float32)
+    if kind == "small":       # every V some 1e-3, the tail's too
+        V *= 1e-3
+    elif kind == "tiny":
+        V *= 1e-4
+    elif kind == "zeros":     # a block of zeros, one of negative zeros, and a head that is all zeros
+        V *= 1e-3
+        V[96:128], V[160:192, 0], V[:, 1] = 0, -0.0, 0
+    elif kind == "zeros, tiny":
+        V *= 1e-4
+        V[64:128], V[:32, 1] = 0, 0
+    elif kind == "zero tail":
+        V[n // BLOCK * BLOCK - BLOCK:] = 0
+        V *= 1e-3
+    elif kind == "outlier":   # one key of V 1e4 times the others', with no weight
+        V *= 1e-2
+        V[70] *= 1e4
+        q[:, :, 0], K[:, :, 0], K[70, :, 0] = 4, 0, -8 * np.sqrt(d)
+    elif kind == "large":     # up to the largest fp16, the infinities beyond it stored as that
+        V *= 2e4
+    with np.errstate(over="ignore"):
+        return K.astype(np.float16), V.astype(np.float16), q.astype(np.float16)
+
+
+SMALL = ["small", "tiny", "zeros", "zeros, tiny", "zero tail", "outlier", "large"]
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("kind", SMALL)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("m", [1, 3, 16])
+def test_attention_small_v(la, synth, cuda, fmt, kind, d, m):
+    import torch
+
+    ctx, qh, kvh = 1500, 8, 2
+    K, V, q = small(synth, kind, ctx + m, m, qh, kvh, d)
+    cache = build(la, cuda, fmt, K, V, ctx)
+    sealed = ctx // BLOCK * BLOCK
+    want, wl = attention64(q, values(K, sealed, fmt), values(V, sealed, fmt), ctx)
+    for splits in (0, 1, 5):
+        lse = torch.empty((m, qh), dtype=torch.float32, device=cuda)
+        got = cache.verify(dev(q, cuda), ctx, splits=splits, lse=lse)
+        la.sync()
+        assert rel_err(got.cpu().numpy(), want) < TOL, splits
+        assert np.max(np.abs(lse.cpu().numpy() - wl) / np.maximum(1, np.abs(wl))) < TOL_LSE, splits
+        if kind == "zeros":
+            assert not got[:, qh // 2:].any()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("kind", SMALL)
+@pytest.mark.parametrize("qh,kvh,d,ctx,t,window", [
+    (8, 2, 64, 900, 90, 0), (8, 2, 128, 900, 90, 0), (8, 2, 64, 900, 70, 300), (8, 2, 128, 3000, 40, 0)])
+def test_prefill_small_v(la, synth, cuda, fmt, kind, qh, kvh, d, ctx, t, window):
+    n = ctx + t
+    K, V, q = small(synth, kind, n, t, qh, kvh, d)
+    cache = build(la, cuda, fmt, K, V, n)
+    got = cache.prefill(dev(q, cuda), ctx, window=window)
+    la.sync()
+    sealed = n // BLOCK * BLOCK
+    want, _ = attention64(q, values(K, sealed, fmt), values(V, sealed, fmt), ctx, window)
+    assert rel_err(got.cpu().numpy(), want) < TOL
+    if kind == "zeros":
+        assert not got[:, qh // 2:].any()
