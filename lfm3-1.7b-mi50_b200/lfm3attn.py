@@ -540,17 +540,21 @@ class LayerCache8:
 
     def append(self, k, v, pos0: int | None = None, rope=None, k_norm=None, token_stride: int = 0, draft: bool = False,
                stream=None) -> None:
-        """Stores k, v ([n][kv_heads][head_dim] fp16 device tensors, tokens strided alike) at positions pos0.. (default:
-        the end). draft: the new tokens may be rolled back, so only tokens below pos0 are sealed."""
+        """Stores k, v ([n][kv_heads][head_dim] fp16 device tensors, tokens strided alike and apart; token_stride, if
+        given, is that stride) at positions pos0.. (default: the end). draft: the new tokens may be rolled back, so only
+        tokens below pos0 are sealed."""
         pos0 = self.length if pos0 is None else pos0
         n, row = k.shape[0], self.kv_heads * self.head_dim
         if k.dtype != self._f16 or v.dtype != self._f16 or k.shape != v.shape or k.numel() != n * row or not (
                 k.is_cuda and v.is_cuda):
             raise LFM3AError(EINVAL, "k and v must be fp16 [n][kv_heads][head_dim] on the GPU")
-        if not (k.is_contiguous() and v.is_contiguous()) and n > 0:
-            if not (k[0].is_contiguous() and v[0].is_contiguous()) or k.stride(0) != v.stride(0) and n > 1:
-                raise LFM3AError(EINVAL, "k and v need contiguous rows and one token stride")
-            token_stride = token_stride or max(row, k.stride(0))
+        if n > 0 and not (k.is_contiguous() and v.is_contiguous() or k[0].is_contiguous() and v[0].is_contiguous()):
+            raise LFM3AError(EINVAL, "k and v need contiguous rows")
+        if n > 1:   # one token's stride is never used
+            stride = k.stride(0)
+            if stride < row or v.stride(0) != stride or token_stride not in (0, stride):
+                raise LFM3AError(EINVAL, "k and v need one token stride of kv_heads * head_dim or more")
+            token_stride = stride
         if pos0 + n > self.capacity:
             raise LFM3AError(EINVAL, "append past the cache capacity")
         if pos0 > self.length:
@@ -581,6 +585,8 @@ class LayerCache8:
         st, sh, sd = q.stride()
         if q.dtype != self._f16 or not q.is_cuda or d != self.head_dim or sd != 1 or (qh > 1 and sh != d):
             raise LFM3AError(EINVAL, "q must be fp16 [tokens][q_heads][head_dim] on the GPU with contiguous rows")
+        if m > 1 and st < qh * d:
+            raise LFM3AError(EINVAL, "q needs a token stride of q_heads * head_dim or more")
         if ctx_len < 0 or ctx_len + m > self.length:
             raise LFM3AError(EINVAL, "the queries' tokens must be appended first")
         return m, qh, st if m > 1 else qh * d

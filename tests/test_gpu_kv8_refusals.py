@@ -1,0 +1,58 @@
+"""More of what LayerCache8 refuses before any launch, because a kernel would read or write outside the tensors given."""
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture()
+def cache(la, cuda):
+    import torch
+
+    c = la.LayerCache8(la.MODE_I8BLK, 2, 64, 256, device=cuda)
+    x = torch.randn(100, 2, 64, device=cuda).half()
+    c.append(x, x)
+    return c
+
+
+def refused(la, f):
+    with pytest.raises(la.LFM3AError) as e:
+        f()
+    assert e.value.code == la.EINVAL
+
+
+def test_append_token_strides(la, cuda, cache):
+    """A stride of 0 (expand), one below a row, one that the tensors do not have."""
+    import torch
+
+    one = torch.randn(1, 2, 64, device=cuda).half()
+    x = torch.randn(8, 2, 64, device=cuda).half()
+    flat = torch.randn(2000, device=cuda).half()
+    wide = torch.randn(8, 6, 64, device=cuda).half()
+    overlap = flat.as_strided((8, 2, 64), (64, 64, 1))
+    for k, v in ((one.expand(8, 2, 64), one.expand(8, 2, 64)), (x, one.expand(8, 2, 64)), (one.expand(8, 2, 64), x),
+                 (overlap, overlap), (wide[:, :2], x)):
+        refused(la, lambda: cache.append(k, v))
+    for stride in (64, 4096, -128):
+        refused(la, lambda: cache.append(x, x, token_stride=stride))
+    refused(la, lambda: cache.append(wide[:, :2], wide[:, 2:4], token_stride=128))
+    assert (cache.length, cache.sealed) == (100, 96)
+    cache.append(wide[:, :2], wide[:, 2:4], token_stride=384)
+    cache.append(one.expand(1, 2, 64), wide[:1, 2:4])   # a single token has no stride
+    k, v = cache.read(100, 9)
+    la.sync()
+    assert torch.equal(k, torch.cat([wide[:, :2], one])) and torch.equal(v, torch.cat([wide[:, 2:4], wide[:1, 2:4]]))
+
+
+def test_query_token_strides(la, cuda, cache):
+    import torch
+
+    one = torch.randn(1, 8, 64, device=cuda).half()
+    flat = torch.randn(4000, device=cuda).half()
+    lse = torch.zeros(4, 8, device=cuda)
+    for q in (one.expand(4, 8, 64), flat.as_strided((4, 8, 64), (64, 64, 1))):
+        refused(la, lambda: cache.verify(q, 96))
+        refused(la, lambda: cache.prefill(q, 96))
+        refused(la, lambda: cache.key_weights(q, lse, 96))
+    a, b = cache.verify(one.expand(1, 8, 64), 99), cache.verify(one.clone(), 99)
+    la.sync()
+    assert torch.equal(a, b)
