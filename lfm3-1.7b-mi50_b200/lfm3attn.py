@@ -541,8 +541,9 @@ class LayerCache8:
     def append(self, k, v, pos0: int | None = None, rope=None, k_norm=None, token_stride: int = 0, draft: bool = False,
                stream=None) -> None:
         """Stores k, v ([n][kv_heads][head_dim] fp16 device tensors, tokens strided alike and apart; token_stride, if
-        given, is that stride) at positions pos0.. (default: the end). draft: the new tokens may be rolled back, so only
-        tokens below pos0 are sealed."""
+        given, is that stride) at positions pos0.. (default: the end). rope: an fp16 device copy of a rope_table with a
+        row for each of the positions 0 .. pos0 + n - 1. draft: the new tokens may be rolled back, so only tokens below
+        pos0 are sealed."""
         pos0 = self.length if pos0 is None else pos0
         n, row = k.shape[0], self.kv_heads * self.head_dim
         if k.dtype != self._f16 or v.dtype != self._f16 or k.shape != v.shape or k.numel() != n * row or not (
@@ -559,6 +560,12 @@ class LayerCache8:
             raise LFM3AError(EINVAL, "append past the cache capacity")
         if pos0 > self.length:
             raise LFM3AError(EINVAL, "append would leave a gap")
+        if rope is not None and (rope.dtype != self._f16 or not rope.is_cuda or not rope.is_contiguous()
+                                 or rope.dim() != 2 or rope.shape[1] != self.head_dim or rope.shape[0] < pos0 + n):
+            raise LFM3AError(EINVAL, "rope must be a contiguous fp16 [>= pos0 + n][head_dim] table on the GPU")
+        if k_norm is not None and (k_norm.dtype != self._f16 or not k_norm.is_cuda or not k_norm.is_contiguous()
+                                   or k_norm.numel() != self.head_dim):
+            raise LFM3AError(EINVAL, "k_norm must be contiguous fp16 [head_dim] on the GPU")
         seal_to = pos0 if draft else pos0 + n
         _check(self._append(self._view, _ptr(k), _ptr(v), token_stride, pos0, n, self.sealed, seal_to, _ptr(rope),
                             _ptr(k_norm), _stream(stream)))

@@ -56,3 +56,26 @@ def test_query_token_strides(la, cuda, cache):
     a, b = cache.verify(one.expand(1, 8, 64), 99), cache.verify(one.clone(), 99)
     la.sync()
     assert torch.equal(a, b)
+
+
+def test_append_rope_and_norm(la, cuda, cache):
+    """A RoPE table has a row for every position up to the last new one; a norm has head_dim weights."""
+    import torch
+
+    x = torch.randn(8, 2, 64, device=cuda).half()
+    table = torch.from_numpy(la.rope_table(1e6, 1.0, 64, 216)).view(torch.float16).to(cuda)
+    rope = table[:108]
+    for bad in (table[:107], table[:0], table[::2], rope.float(), rope.view(torch.int16), rope.cpu(), rope[:, :32],
+                rope.flatten(), table.view(108, 128), rope.t().contiguous().t()):
+        refused(la, lambda: cache.append(x, x, rope=bad))
+        refused(la, lambda: cache.append(x, x, rope=bad, draft=True))
+    norm = torch.ones(64, device=cuda).half()
+    for bad in (norm[:32], norm.float(), norm.cpu(), torch.ones(128, device=cuda).half()[::2]):
+        refused(la, lambda: cache.append(x, x, k_norm=bad))
+    assert (cache.length, cache.sealed) == (100, 96)
+    cache.append(x, x, rope=rope, k_norm=norm, draft=True)   # the table's last row is the last token's
+    k, _ = cache.read(100, 8)
+    cache.append(x, x, pos0=100, rope=table, k_norm=norm, draft=True)
+    k2, _ = cache.read(100, 8)
+    la.sync()
+    assert torch.equal(k, k2)
