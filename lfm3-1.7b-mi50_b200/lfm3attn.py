@@ -190,8 +190,9 @@ def _ptr(t) -> int | None:
     return t.data_ptr()
 
 
-def _stream(stream) -> int | None:
-    if stream is None:
+def _stream(stream, gpu: int = -1) -> int | None:
+    """The stream's handle. gpu: the device that holds the call's memory, which has to be the current one."""
+    if stream is None or gpu >= 0:
         global _torch, _raw_stream
         if _torch is None:
             import torch
@@ -201,9 +202,11 @@ def _stream(stream) -> int | None:
             raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
             if raw is not None:
                 _raw_stream = raw
-        if _raw_stream is not None:
-            return _raw_stream(_torch.cuda.current_device())
-        return _torch.cuda.current_stream().cuda_stream
+        device = _torch.cuda.current_device()
+        if gpu >= 0 and device != gpu:
+            raise LFM3AError(EINVAL, f"the memory is on GPU {gpu}, which is not the current one")
+        if stream is None:
+            return _raw_stream(device) if _raw_stream is not None else _torch.cuda.current_stream().cuda_stream
     if isinstance(stream, int):
         return stream
     return stream.cuda_stream
@@ -489,7 +492,8 @@ class LayerCache8:
 
     def __init__(self, mode: int, kv_heads: int, head_dim: int, capacity_tokens: int, device="cuda", block_table=None,
                  pool_blocks: int | None = None, pool=None):
-        """pool: another LayerCache8 of the same layout whose pool this one shares through its own block table."""
+        """pool: another LayerCache8 of the same layout whose pool this one shares through its own block table.
+        Every tensor of a call has to be on the cache's GPU, which has to be the current one."""
         import torch
 
         if mode not in (MODE_I8BLK, MODE_E4M3BLK):
@@ -511,6 +515,9 @@ class LayerCache8:
             raise LFM3AError(EINVAL, "block_table must hold an int32 for every 32 tokens of the capacity")
         self.table = block_table
         self.tail = torch.zeros(lib().lfm3a_kv8_tail_bytes(ctypes.byref(self.layout)), dtype=torch.uint8, device=device)
+        self._gpu = self.pool.get_device()
+        if self._gpu < 0 or self.table.get_device() != self._gpu or self.tail.get_device() != self._gpu:
+            raise LFM3AError(EINVAL, "pool, block_table and tail must be on one GPU")
         self.length = self.sealed = 0
         self.view = Kv8View(KvView(self.pool.data_ptr(), self.table.data_ptr(), self.pool_blocks, self.layout),
                             self.tail.data_ptr())
@@ -547,8 +554,8 @@ class LayerCache8:
         pos0 = self.length if pos0 is None else pos0
         n, row = k.shape[0], self.kv_heads * self.head_dim
         if k.dtype != self._f16 or v.dtype != self._f16 or k.shape != v.shape or k.numel() != n * row or not (
-                k.is_cuda and v.is_cuda):
-            raise LFM3AError(EINVAL, "k and v must be fp16 [n][kv_heads][head_dim] on the GPU")
+                k.get_device() == v.get_device() == self._gpu):
+            raise LFM3AError(EINVAL, "k and v must be fp16 [n][kv_heads][head_dim] on the cache's GPU")
         if n > 0 and not (k.is_contiguous() and v.is_contiguous() or k[0].is_contiguous() and v[0].is_contiguous()):
             raise LFM3AError(EINVAL, "k and v need contiguous rows")
         if n > 1:   # one token's stride is never used
@@ -560,15 +567,15 @@ class LayerCache8:
             raise LFM3AError(EINVAL, "append past the cache capacity")
         if pos0 > self.length:
             raise LFM3AError(EINVAL, "append would leave a gap")
-        if rope is not None and (rope.dtype != self._f16 or not rope.is_cuda or not rope.is_contiguous()
+        if rope is not None and (rope.dtype != self._f16 or rope.get_device() != self._gpu or not rope.is_contiguous()
                                  or rope.dim() != 2 or rope.shape[1] != self.head_dim or rope.shape[0] < pos0 + n):
-            raise LFM3AError(EINVAL, "rope must be a contiguous fp16 [>= pos0 + n][head_dim] table on the GPU")
-        if k_norm is not None and (k_norm.dtype != self._f16 or not k_norm.is_cuda or not k_norm.is_contiguous()
+            raise LFM3AError(EINVAL, "rope must be a contiguous fp16 [>= pos0 + n][head_dim] table on the cache's GPU")
+        if k_norm is not None and (k_norm.dtype != self._f16 or k_norm.get_device() != self._gpu or not k_norm.is_contiguous()
                                    or k_norm.numel() != self.head_dim):
-            raise LFM3AError(EINVAL, "k_norm must be contiguous fp16 [head_dim] on the GPU")
+            raise LFM3AError(EINVAL, "k_norm must be contiguous fp16 [head_dim] on the cache's GPU")
         seal_to = pos0 if draft else pos0 + n
         _check(self._append(self._view, _ptr(k), _ptr(v), token_stride, pos0, n, self.sealed, seal_to, _ptr(rope),
-                            _ptr(k_norm), _stream(stream)))
+                            _ptr(k_norm), _stream(stream, self._gpu)))
         self.sealed = seal_to // BLOCK_TOKENS * BLOCK_TOKENS
         self.length = pos0 + n
 
@@ -584,14 +591,14 @@ class LayerCache8:
             raise LFM3AError(EINVAL, "read past the cached tokens")
         k = self.tail.new_empty((n, self.kv_heads, self.head_dim), dtype=self._f16)
         v = self._like(k)
-        _check(self._read(self._view, pos0, n, self.sealed, k.data_ptr(), v.data_ptr(), _stream(stream)))
+        _check(self._read(self._view, pos0, n, self.sealed, k.data_ptr(), v.data_ptr(), _stream(stream, self._gpu)))
         return k, v
 
     def _check_q(self, q, ctx_len: int) -> tuple[int, int, int]:
         m, qh, d = q.shape
         st, sh, sd = q.stride()
-        if q.dtype != self._f16 or not q.is_cuda or d != self.head_dim or sd != 1 or (qh > 1 and sh != d):
-            raise LFM3AError(EINVAL, "q must be fp16 [tokens][q_heads][head_dim] on the GPU with contiguous rows")
+        if q.dtype != self._f16 or q.get_device() != self._gpu or d != self.head_dim or sd != 1 or (qh > 1 and sh != d):
+            raise LFM3AError(EINVAL, "q must be fp16 [tokens][q_heads][head_dim] on the cache's GPU with contiguous rows")
         if m > 1 and st < qh * d:
             raise LFM3AError(EINVAL, "q needs a token stride of q_heads * head_dim or more")
         if ctx_len < 0 or ctx_len + m > self.length:
@@ -599,12 +606,16 @@ class LayerCache8:
         return m, qh, st if m > 1 else qh * d
 
     def _check_f16(self, shape, t) -> None:
-        if t.dtype != self._f16 or t.shape != shape or not t.is_contiguous() or not t.is_cuda:
-            raise LFM3AError(EINVAL, "gate [m][q_heads] and out (q's shape) must be contiguous fp16 on the GPU")
+        if t.dtype != self._f16 or t.shape != shape or not t.is_contiguous() or t.get_device() != self._gpu:
+            raise LFM3AError(EINVAL, "gate [m][q_heads] and out (q's shape) must be contiguous fp16 on the cache's GPU")
 
     def _check_lse(self, lse, m: int, qh: int) -> None:
-        if lse.dtype != self._f32 or lse.shape != (m, qh) or not lse.is_contiguous() or not lse.is_cuda:
-            raise LFM3AError(EINVAL, "lse must be fp32 [m][q_heads] on the GPU")
+        if lse.dtype != self._f32 or lse.shape != (m, qh) or not lse.is_contiguous() or lse.get_device() != self._gpu:
+            raise LFM3AError(EINVAL, "lse must be fp32 [m][q_heads] on the cache's GPU")
+
+    def _check_workspace(self, workspace) -> None:
+        if workspace.get_device() != self._gpu or not workspace.is_contiguous():
+            raise LFM3AError(EINVAL, "workspace must be contiguous on the cache's GPU")
 
     def verify(self, q, ctx_len: int, window: int = 0, gate=None, out=None, lse=None, workspace=None, splits: int = 0,
                stream=None):
@@ -622,9 +633,11 @@ class LayerCache8:
         if workspace is None:
             s = splits if splits > 0 else self.splits(qh, ctx_len, m, window)
             workspace = q.new_empty(lib().lfm3a_verify_workspace_bytes(m, qh, self.head_dim, s) // 4, dtype=self._f32)
+        else:
+            self._check_workspace(workspace)
         _check(self._attention(self._view, q.data_ptr(), stride, m, qh, ctx_len, self.sealed_below(ctx_len + m), window,
                                _ptr(gate), out.data_ptr(), _ptr(lse), workspace.data_ptr(), workspace.nbytes, splits,
-                               _stream(stream)))
+                               _stream(stream, self._gpu)))
         return out
 
     def sealed_below(self, length: int) -> int:
@@ -647,8 +660,10 @@ class LayerCache8:
             workspace = torch.empty(lib().lfm3a_kv8_prefill_workspace_bytes(ctypes.byref(self.layout), t, qh,
                                                                             context + t), dtype=torch.uint8,
                                     device=q.device)
+        else:
+            self._check_workspace(workspace)
         _check(lib().lfm3a_kv8_prefill(self._view, _ptr(q), stride, t, qh, context, self.sealed_below(context + t), window,
-                                       _ptr(out), _ptr(workspace), workspace.numel(), _stream(stream)))
+                                       _ptr(out), _ptr(workspace), workspace.nbytes, _stream(stream, self._gpu)))
         return out
 
     def key_weights(self, q, lse, ctx_len: int, window: int = 0, prev=None, decay: float = 1.0, out=None, stream=None):
@@ -661,11 +676,11 @@ class LayerCache8:
             out = q.new_empty((self.kv_heads, n), dtype=self._f32)
         for t in (out, prev):
             if t is not None and (t.dtype != self._f32 or t.shape[0] != self.kv_heads or t.shape[1] < n or t.stride(1) != 1
-                                  or not t.is_cuda):
-                raise LFM3AError(EINVAL, "weights must be fp32 [kv_heads][>= ctx_len + m] on the GPU")
+                                  or t.get_device() != self._gpu):
+                raise LFM3AError(EINVAL, "weights must be fp32 [kv_heads][>= ctx_len + m] on the cache's GPU")
         _check(self._weights(self._view, q.data_ptr(), stride, m, qh, ctx_len, self.sealed_below(n), window,
                              lse.data_ptr(), _ptr(prev), 0 if prev is None else prev.stride(0), decay, out.data_ptr(),
-                             out.stride(0), _stream(stream)))
+                             out.stride(0), _stream(stream, self._gpu)))
         return out
 
     def evict(self, weights, budget: int, sink: int, recent: int, dst: "LayerCache8", stream=None):
@@ -676,8 +691,10 @@ class LayerCache8:
             raise LFM3AError(EINVAL, "eviction needs another cache with room for the budget")
         if weights.shape[0] != self.kv_heads or dst.mode != self.mode or dst.layout.block_bytes != self.layout.block_bytes:
             raise LFM3AError(EINVAL, "eviction needs weights of each kv head and a cache of the same layout")
+        if not weights.get_device() == dst._gpu == self._gpu:
+            raise LFM3AError(EINVAL, "eviction needs weights and a cache on this cache's GPU")
         keep, kept = evict_select(weights, self.length, budget, sink, recent, stream=stream)
-        _check(self._compact(self._view, self.length, self.sealed, keep.data_ptr(), budget, dst._view, _stream(stream)))
+        _check(self._compact(self._view, self.length, self.sealed, keep.data_ptr(), budget, dst._view, _stream(stream, self._gpu)))
         dst.length, dst.sealed = budget, budget // BLOCK_TOKENS * BLOCK_TOKENS
         return keep, kept
 
@@ -693,7 +710,7 @@ def evict_select(weights, length: int, budget: int, sink: int, recent: int, stre
     kept = weights.new_empty((h, max(0, budget)))
     keep = torch.empty_like(kept, dtype=torch.int32)
     _check(lib().lfm3a_evict_select(weights.data_ptr(), row, h, length, sink, recent, budget, keep.data_ptr(),
-                                    kept.data_ptr(), kept.stride(0), _stream(stream)))
+                                    kept.data_ptr(), kept.stride(0), _stream(stream, weights.get_device())))
     return keep, kept
 
 

@@ -79,3 +79,52 @@ def test_append_rope_and_norm(la, cuda, cache):
     k2, _ = cache.read(100, 8)
     la.sync()
     assert torch.equal(k, k2)
+
+
+def test_memory_of_another_device(la, cuda, cache, monkeypatch):
+    """Tensors on the host, and on a GPU that is not the cache's (here the cache takes itself to be on GPU 1)."""
+    import torch
+
+    def make(**kw):
+        return la.LayerCache8(la.MODE_I8BLK, 2, 64, 256, **kw)
+
+    refused(la, lambda: make(device=cuda, block_table=torch.arange(8, dtype=torch.int32)))
+    refused(la, lambda: make(device="cpu"))
+    refused(la, lambda: make(device="cpu", pool=cache, block_table=torch.arange(8, dtype=torch.int32, device=cuda)))
+    q = torch.randn(4, 8, 64, device=cuda).half()
+    ws = torch.empty(1 << 22, dtype=torch.uint8, device=cuda)
+    for bad in (ws.cpu(), ws.view(2048, 2048).t()):
+        refused(la, lambda: cache.verify(q, 96, workspace=bad))
+        refused(la, lambda: cache.prefill(q, 96, workspace=bad))
+
+    x = torch.randn(8, 2, 64, device=cuda).half()
+    rope = torch.zeros(108, 64, device=cuda).half()
+    lse, w = torch.zeros(4, 8, device=cuda), torch.zeros(2, 100, device=cuda)
+    dst, other = make(device=cuda), make(device=cuda)
+    calls = [lambda c: c.append(x, x), lambda c: c.append(x, x, rope=rope), lambda c: c.append(x, x, k_norm=rope[0]),
+             lambda c: c.read(0, 4), lambda c: c.verify(q, 96), lambda c: c.verify(q, 96, workspace=ws),
+             lambda c: c.prefill(q, 96), lambda c: c.key_weights(q, lse, 96), lambda c: c.evict(w, 40, 1, 2, dst)]
+    monkeypatch.setattr(other, "_gpu", 1)
+    other.length, other.sealed = cache.length, cache.sealed
+    side = torch.cuda.Stream()
+    for call in calls:
+        refused(la, lambda: call(other))
+    refused(la, lambda: cache.evict(w, 40, 1, 2, other))
+    refused(la, lambda: other.read(0, 4, stream=side))
+    refused(la, lambda: other.read(0, 4, stream=side.cuda_stream))
+    assert (other.length, dst.length) == (100, 0)
+    for call in calls:   # the same calls are right on the cache's own GPU
+        call(cache)
+        cache.truncate(100)
+    la.sync()
+
+
+def test_current_device(la, cuda, cache, monkeypatch):
+    """A call while another GPU is the current one would launch there."""
+    import torch
+
+    w = torch.zeros(2, 100, device=cuda)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    refused(la, lambda: cache.read(0, 4))
+    refused(la, lambda: cache.read(0, 4, stream=0))
+    refused(la, lambda: la.evict_select(w, 100, 40, 1, 2))
