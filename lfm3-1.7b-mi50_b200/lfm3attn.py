@@ -683,16 +683,30 @@ class LayerCache8:
                              out.stride(0), _stream(stream, self._gpu)))
         return out
 
+    def _check_apart(self, dst: "LayerCache8", budget: int) -> None:
+        """The blocks that compaction writes are none of those that it reads (the kernels keep entries within the pool)."""
+        import torch
+
+        if torch.cuda.is_current_stream_capturing():
+            raise LFM3AError(EINVAL, "eviction within a pool looks at the block tables, which a capture cannot")
+        read = self.table[:self.sealed // BLOCK_TOKENS].clamp(0, self.pool_blocks - 1)
+        written = dst.table[:budget // BLOCK_TOKENS].clamp(0, self.pool_blocks - 1)
+        if torch.isin(written, read).any():
+            raise LFM3AError(EINVAL, "eviction into blocks of the pool that this cache still holds")
+
     def evict(self, weights, budget: int, sink: int, recent: int, dst: "LayerCache8", stream=None):
         """Keeps `budget` tokens of each kv head (the first `sink`, the last `recent`, the heaviest others by
         weights [kv_heads][>= length]) and moves them into dst, whose earlier content is replaced. Returns
-        (keep int32 [kv_heads][budget], the kept keys' weights)."""
+        (keep int32 [kv_heads][budget], the kept keys' weights). dst may share this cache's pool, through other blocks:
+        that the two tables have none in common is looked up on the host, which waits for the GPU."""
         if dst is self or budget > dst.capacity:
             raise LFM3AError(EINVAL, "eviction needs another cache with room for the budget")
         if weights.shape[0] != self.kv_heads or dst.mode != self.mode or dst.layout.block_bytes != self.layout.block_bytes:
             raise LFM3AError(EINVAL, "eviction needs weights of each kv head and a cache of the same layout")
         if not weights.get_device() == dst._gpu == self._gpu:
             raise LFM3AError(EINVAL, "eviction needs weights and a cache on this cache's GPU")
+        if dst.pool.data_ptr() == self.pool.data_ptr():
+            self._check_apart(dst, budget)
         keep, kept = evict_select(weights, self.length, budget, sink, recent, stream=stream)
         _check(self._compact(self._view, self.length, self.sealed, keep.data_ptr(), budget, dst._view, _stream(stream, self._gpu)))
         dst.length, dst.sealed = budget, budget // BLOCK_TOKENS * BLOCK_TOKENS
