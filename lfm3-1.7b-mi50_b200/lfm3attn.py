@@ -212,6 +212,22 @@ def _stream(stream, gpu: int = -1) -> int | None:
     return stream.cuda_stream
 
 
+def _on(stream, gpu: int, call, *args):
+    """call(*args) with `stream` as torch's current stream, so that what it allocates belongs to that stream and is not
+    reused elsewhere while its kernels run; what it returns is kept until the caller's stream is through with it, too."""
+    _stream(stream, gpu)
+    import torch
+
+    if isinstance(stream, int):
+        stream = torch.cuda.ExternalStream(stream) if stream else torch.cuda.default_stream()
+    caller = torch.cuda.current_stream()
+    with torch.cuda.stream(stream):
+        got = call(*args)
+    for t in got if isinstance(got, tuple) else (got,):
+        t.record_stream(caller)
+    return got
+
+
 def layout(mode: int, kv_heads: int, head_dim: int, block_tokens: int = BLOCK_TOKENS) -> KvLayout:
     out = KvLayout()
     _check(lib().lfm3a_kv_layout_init(mode, kv_heads, head_dim, block_tokens, ctypes.byref(out)))
@@ -488,7 +504,10 @@ class LayerCache8:
     kv head), its block table and the fp16 tail of the tokens that are not sealed yet (include/lfm3attn.h).
 
     `length` tokens are cached, `sealed` of them in 8 bits. append seals every complete block of committed tokens;
-    tokens appended as drafts stay in the tail until a later append finds them committed (below its position)."""
+    tokens appended as drafts stay in the tail until a later append finds them committed (below its position).
+
+    A call with stream= runs on that stream, with its workspace and results allocated there: its inputs have to be ready
+    on that stream, and the caller's stream has to wait for it before it uses the results."""
 
     def __init__(self, mode: int, kv_heads: int, head_dim: int, capacity_tokens: int, device="cuda", block_table=None,
                  pool_blocks: int | None = None, pool=None):
@@ -589,9 +608,11 @@ class LayerCache8:
         """(K, V) fp16 [n][kv_heads][head_dim]: the values the cached tokens pos0.. stand for."""
         if pos0 < 0 or n < 0 or pos0 + n > self.length:
             raise LFM3AError(EINVAL, "read past the cached tokens")
+        if stream is not None:
+            return _on(stream, self._gpu, self.read, pos0, n)
         k = self.tail.new_empty((n, self.kv_heads, self.head_dim), dtype=self._f16)
         v = self._like(k)
-        _check(self._read(self._view, pos0, n, self.sealed, k.data_ptr(), v.data_ptr(), _stream(stream, self._gpu)))
+        _check(self._read(self._view, pos0, n, self.sealed, k.data_ptr(), v.data_ptr(), _stream(None, self._gpu)))
         return k, v
 
     def _check_q(self, q, ctx_len: int) -> tuple[int, int, int]:
@@ -621,6 +642,8 @@ class LayerCache8:
                stream=None):
         """Attention of q ([m][q_heads][head_dim] fp16, row-strided) at ctx_len.., m <= 32; the tokens' K/V appended.
         lse: fp32 [m][q_heads] to fill with each row's log-sum-exp. Returns fp16 [m][q_heads][head_dim]."""
+        if stream is not None:
+            return _on(stream, self._gpu, self.verify, q, ctx_len, window, gate, out, lse, workspace, splits)
         m, qh, stride = self._check_q(q, ctx_len)
         if gate is not None:
             self._check_f16((m, qh), gate)
@@ -637,7 +660,7 @@ class LayerCache8:
             self._check_workspace(workspace)
         _check(self._attention(self._view, q.data_ptr(), stride, m, qh, ctx_len, self.sealed_below(ctx_len + m), window,
                                _ptr(gate), out.data_ptr(), _ptr(lse), workspace.data_ptr(), workspace.nbytes, splits,
-                               _stream(stream, self._gpu)))
+                               _stream(None, self._gpu)))
         return out
 
     def sealed_below(self, length: int) -> int:
@@ -647,6 +670,8 @@ class LayerCache8:
     def prefill(self, q, context: int, window: int = 0, out=None, workspace=None, stream=None):
         """Causal attention of a prompt chunk q ([T][q_heads][head_dim] fp16, row-strided) at context.., appended
         before."""
+        if stream is not None:
+            return _on(stream, self._gpu, self.prefill, q, context, window, out, workspace)
         import torch
 
         t, qh, stride = self._check_q(q, context)
@@ -663,12 +688,14 @@ class LayerCache8:
         else:
             self._check_workspace(workspace)
         _check(lib().lfm3a_kv8_prefill(self._view, _ptr(q), stride, t, qh, context, self.sealed_below(context + t), window,
-                                       _ptr(out), _ptr(workspace), workspace.nbytes, _stream(stream, self._gpu)))
+                                       _ptr(out), _ptr(workspace), workspace.nbytes, _stream(None, self._gpu)))
         return out
 
     def key_weights(self, q, lse, ctx_len: int, window: int = 0, prev=None, decay: float = 1.0, out=None, stream=None):
         """fp32 [kv_heads][ctx_len + m]: decay * prev plus the attention weight each key got from the m tokens of q,
         summed over the query heads of its kv head. lse: of verify for the same q."""
+        if stream is not None:
+            return _on(stream, self._gpu, self.key_weights, q, lse, ctx_len, window, prev, decay, out)
         m, qh, stride = self._check_q(q, ctx_len)
         self._check_lse(lse, m, qh)
         n = ctx_len + m
@@ -680,7 +707,7 @@ class LayerCache8:
                 raise LFM3AError(EINVAL, "weights must be fp32 [kv_heads][>= ctx_len + m] on the cache's GPU")
         _check(self._weights(self._view, q.data_ptr(), stride, m, qh, ctx_len, self.sealed_below(n), window,
                              lse.data_ptr(), _ptr(prev), 0 if prev is None else prev.stride(0), decay, out.data_ptr(),
-                             out.stride(0), _stream(stream, self._gpu)))
+                             out.stride(0), _stream(None, self._gpu)))
         return out
 
     def _check_apart(self, dst: "LayerCache8", budget: int) -> None:
@@ -699,6 +726,8 @@ class LayerCache8:
         weights [kv_heads][>= length]) and moves them into dst, whose earlier content is replaced. Returns
         (keep int32 [kv_heads][budget], the kept keys' weights). dst may share this cache's pool, through other blocks:
         that the two tables have none in common is looked up on the host, which waits for the GPU."""
+        if stream is not None:
+            return _on(stream, self._gpu, self.evict, weights, budget, sink, recent, dst)
         if dst is self or budget > dst.capacity:
             raise LFM3AError(EINVAL, "eviction needs another cache with room for the budget")
         if weights.shape[0] != self.kv_heads or dst.mode != self.mode or dst.layout.block_bytes != self.layout.block_bytes:
@@ -707,8 +736,9 @@ class LayerCache8:
             raise LFM3AError(EINVAL, "eviction needs weights and a cache on this cache's GPU")
         if dst.pool.data_ptr() == self.pool.data_ptr():
             self._check_apart(dst, budget)
-        keep, kept = evict_select(weights, self.length, budget, sink, recent, stream=stream)
-        _check(self._compact(self._view, self.length, self.sealed, keep.data_ptr(), budget, dst._view, _stream(stream, self._gpu)))
+        keep, kept = evict_select(weights, self.length, budget, sink, recent)
+        _check(self._compact(self._view, self.length, self.sealed, keep.data_ptr(), budget, dst._view,
+                             _stream(None, self._gpu)))
         dst.length, dst.sealed = budget, budget // BLOCK_TOKENS * BLOCK_TOKENS
         return keep, kept
 
@@ -717,6 +747,8 @@ def evict_select(weights, length: int, budget: int, sink: int, recent: int, stre
     """(keep int32 [kv_heads][budget] ascending, the kept keys' weights fp32) of weights fp32 [kv_heads][>= length]."""
     import torch
 
+    if stream is not None:
+        return _on(stream, weights.get_device(), evict_select, weights, length, budget, sink, recent)
     h, width = weights.shape
     row, one = weights.stride()
     if weights.dtype != torch.float32 or width < length or one != 1 or not weights.is_cuda:
@@ -724,7 +756,7 @@ def evict_select(weights, length: int, budget: int, sink: int, recent: int, stre
     kept = weights.new_empty((h, max(0, budget)))
     keep = torch.empty_like(kept, dtype=torch.int32)
     _check(lib().lfm3a_evict_select(weights.data_ptr(), row, h, length, sink, recent, budget, keep.data_ptr(),
-                                    kept.data_ptr(), kept.stride(0), _stream(stream, weights.get_device())))
+                                    kept.data_ptr(), kept.stride(0), _stream(None, weights.get_device())))
     return keep, kept
 
 
