@@ -721,7 +721,7 @@ __device__ __forceinline__ void kv8_exponents(float (&x)[HB][NT][4], int n, floa
     }
 }
 
-// A warp's running state: O^T accumulators, the maxima of its lanes' rows, the sums of P' / vs, exact and with P' rounded (round11).
+// A warp's running state: O^T accumulators, the maxima of its lanes' rows, the sums of P' / vs, exact and of rounded P'.
 template <int D, int NT>
 struct Kv8Rows {
   float o[D / 16][NT][4];
@@ -810,15 +810,15 @@ __device__ __forceinline__ void kv8_softmax(const QK& qk, Kv8Rows<D, NT>& w, con
 // s + log2 vs less kHeadroom, gives sum P' v8 = 2^-m' sum 2^s v directly, and l = sum P' / vs is the softmax sum, of fp32
 // P': a page of small vs keeps its share of the sum where its P' is below fp16's normal values (round11). m' is lazy (moved
 // only when a score passes it by 2^15; fp16 P then stays within 2^15 and fp32 sums are unaffected), so the common page
-// needs no shuffles but one vote. Open pages come last: their factor of 1 moves m' when the others' P' is summed already. movmatrix turns the S^T accumulators into the B operand of O^T = V^T P.
+// needs no shuffles but one vote. A warp's open pages come last: their factor of 1 moves m' when the others' P' is summed
+// already. movmatrix turns the S^T accumulators into the B operand of O^T = V^T P.
 // The warps meet in shared memory at the end; one split writes its rows, several write (acc, m', l) partials.
-//
-// What bounds it: HBM for one token (100003 tokens at 32/8/64, int8: 21.6 us with the merge, 4.8 TB/s; 131072: 26.6 us),
-// instructions from 2 n-tiles on (some 370 a page and warp at 16 rows, 55% of the issue slots with 16 warps per SM).
+// What bounds it: HBM for one token (100003 tokens at 32/8/64, int8: 21.9 us with the merge, 4.7 TB/s; 131072: 27.0 us),
+// instructions from 2 n-tiles on (some 380 a page and warp at 16 rows, 55% of the issue slots with 16 warps per SM).
 //
 // CLUSTER: the splits of a kv head are a cluster of kKv8Cluster blocks that merge through each other's shared memory, so a
-// short context needs no second launch. Over 777 tokens (int8), one launch against two: 32/8/64, 1 token 5.7 us against
-// 5.6, 4 tokens 7.4 against 8.5; 16/4/128, 6.5 against 6.9 and 9.6 against 10.6; and 2.3 us less of the host's time each.
+// short context needs no second launch. Over 777 tokens (int8), one launch against two: 32/8/64, 1 token 5.8 us against
+// 5.8, 4 tokens 7.2 against 8.4; 16/4/128, 6.6 against 7.1 and 9.4 against 10.7; and 2.3 us less of the host's time each.
 constexpr int kKv8Cluster = 8;
 template <int D, int NT, bool E4M3, bool CLUSTER>
 __device__ __forceinline__ void kv8_attend(const Kv8AttnArgs& a) {
@@ -1142,7 +1142,7 @@ struct Kv8ExpandArgs {
 
 // One page and kv head of the cache as the K and V tiles of a MODE_F16 section, the codes as fp16 (exactly; the scales go
 // beside them): what the prefill kernel's SCALED form reads. Values past the sequence's end are 0. 32000 tokens at 4 heads
-// of 128 take 17 us beside 750 for a chunk of 1999 over them; expanding inside the prefill kernel would repeat the work
+// of 128 take 17 us beside 760 for a chunk of 1999 over them; expanding inside the prefill kernel would repeat the work
 // for each of the chunk's 63 row tiles.
 template <int D, bool E4M3>
 __global__ __launch_bounds__(128) void kv8_expand_kernel(Kv8ExpandArgs a) {
@@ -1239,7 +1239,7 @@ struct Kv8Weights {
 // chain of MMAs for one token (131072 tokens at 32/8/64: 19.2 us with a sum so far, 3.9 TB/s), by the MMAs for many rows.
 // SHARE: in a last round with half of a block's warps or less to do, 2 to 8 warps share a page's rows, and their sums meet
 // in shared memory. It costs the loop some instructions: int8, 32/8/64, 32 tokens over 20000 17.0 us against 19.1 without
-// (2 rounds of pages), 4 tokens over 131000 22.8 against 20.5 (16 rounds), so kv8_weights_share picks it for few rounds.
+// (2 rounds of pages), 4 tokens over 131000 22.8 against 20.5 (14 rounds), so kv8_weights_share picks it for few rounds.
 template <int D, bool E4M3, bool SHARE>
 __global__ __launch_bounds__(Kv8Weights<D>::kThreads, 2) void kv8_weights_kernel(Kv8WeightArgs a) {
   using L = Kv8Weights<D>;

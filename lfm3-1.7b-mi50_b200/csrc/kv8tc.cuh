@@ -19,7 +19,7 @@
 // cycles on each issuing warp, all on 4.5 warps per scheduler; shared memory alone moves 144 KB a tile, 1150 cycles (codes
 // in, codes out, fp16 in, operands out). The warp-level kernel converts in registers and has no such traffic, but its
 // MMAs (8 cycles each per scheduler, 1024 a tile at 64 rows) and 4 times the conversions come to more from 33 rows on.
-// Measured: 16 tokens over 131072 at 32/8/64 (int8) 57.6 us with the merge (2.3 TB/s), against 91 for the other kernel.
+// Measured: 16 tokens over 131072 at 32/8/64 (int8) 59.1 us with the merge (2.3 TB/s), against 92 for the other kernel.
 // The order of keys within a page is free as long as P and V agree: V's 16-byte row c of a dim holds the keys 2c, 2c + 1,
 // 2c + 8, 2c + 9, 16 + 2c, 17 + 2c, 24 + 2c, 25 + 2c, which is how a lane finds them in the cache.
 #pragma once

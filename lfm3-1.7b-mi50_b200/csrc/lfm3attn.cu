@@ -1218,9 +1218,9 @@ int with_format(const lfm3a_kv_layout& L, F f) {
   return e4m3 ? f(std::integral_constant<int, 128>{}, std::true_type{}) : f(std::integral_constant<int, 128>{}, std::false_type{});
 }
 
-// Query rows of one kv head that a block takes: kv8_attend_kernel's 8 or 16, or the 64 of kv8_attend_tc_kernel. 17 to 32 rows
-// go through the former in two groups: over 131072 tokens at 32/8/64 (int8) 51.0 us against 55.7; 48 rows 72 against 57,
-// 64 rows 91 against 58, 128 rows 191 against 105.
+// Query rows of one kv head that a block takes: kv8_attend_kernel's 8 or 16 (17 to 32 go there in two groups), or the 64 of
+// kv8_attend_tc_kernel. Us over 131072 tokens, the former and the latter, at 32, 48, 64 rows: 32/8/64 int8 52 57, 72 58, 92 59,
+// e4m3 48 56, 66 57, 84 57; 16/4/128 int8 45 62, 61 64, 76 65, e4m3 40 60, 54 61, 66 62 (so 33 to 48 rows lose 4-12% there).
 int kv8_rows_per_block(int rows) { return rows <= 8 ? 8 : rows <= 32 ? 16 : 64; }
 
 // Key splits: one wave of resident blocks, at least a page for each of a block's warps (8, 12 at head_dim 128), or a
